@@ -37,3 +37,20 @@ def pytest_configure(config):
 @pytest.fixture(scope="session")
 def golden_dir():
     return GOLDEN
+
+
+CHAINS_NOT_KEPT = (("orth", "6", "20"), ("synth", "7", "20"))
+WHOLE_SET_TESTS = ("test_strict_sam_index_of_the_headline_mode", "test_bench_line_is_the_compact_contract_object")
+
+
+def pytest_collection_modifyitems(config, items):
+    """Two members of the reference-chain set (orth:6:20, synth:7:20) are not kept in the repository (they are regenerated from the
+    reference by tests/golden/make_golden_chains.py): where a file is absent, its cases and the two tests that walk the whole set of
+    eleven are skipped."""
+    import re
+    absent = ["%s_n%s_T%s.npz" % c for c in CHAINS_NOT_KEPT if not os.path.exists(os.path.join(GOLDEN, "chains", "%s_n%s_T%s.npz" % c))]
+    for item in items:
+        m = re.search(r"\b(orth|synth)-n(\d+)-T(\d+)\b", item.name)
+        name = "%s_n%s_T%s.npz" % m.groups() if m else None
+        if absent and (name in absent or item.name in WHOLE_SET_TESTS):
+            item.add_marker(pytest.mark.skip(reason="reference chain not in this checkout: %s" % (name or ", ".join(absent))))
