@@ -17,7 +17,7 @@ BF16, F32X3, F16, F32H = 0, 1, 2, 3      # (F32H: hsidm_conv2d only - ops.Packed
 XF_NONE, XF_AFFINE, XF_AFFINE_SILU = 0, 1, 2
 ACT_NONE, ACT_LEAKY = 0, 1
 
-_vp, _i32, _i64, _u32, _u64, _f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_float
+_vp, _i32, _i64, _u32, _u64, _f32, _f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_float, C.c_double
 
 
 class ConvPhase(C.Structure):
@@ -37,6 +37,10 @@ class ConvDesc(C.Structure):
 class WgradItem(C.Structure):
     _fields_ = [("ws", _vp), ("dw", _vp), ("nsplit", _i32), ("NT", _i32), ("Cout_pad", _i32), ("Cin_pad", _i32), ("Cout_w", _i32),
                 ("Cin_w", _i32), ("block0", _i32), ("layout", _i32)]
+
+
+class TensorItem(C.Structure):
+    _fields_ = [("ptr", _vp), ("n", _i64), ("type", _i32), ("reserved", _i32)]
 
 
 # name -> argtypes, exactly the prototypes of include/hsidm.h
@@ -98,8 +102,12 @@ SIGNATURES = {
     "hsidm_softmax_bwd_rows": [_vp, _vp, _i64, _i32, _f32, _vp],
     "hsidm_gather_pack": [_vp, _vp, _i64, _vp, _vp, _vp],
     "hsidm_adam_step": [_vp, _vp, _vp, _vp, _i64, _f32, _f32, _f32, _f32, _i32, _f32, _vp, _vp],
+    "hsidm_adam_step_clipped": [_vp, _vp, _vp, _vp, _i64, _f32, _f32, _f32, _f32, _i32, _f32, _vp, _vp, _vp],
+    "hsidm_grad_norm_workspace_bytes": [_i32],
+    "hsidm_grad_norm": [C.POINTER(TensorItem), _i32, _f64, _f64, _vp, _vp, _vp],
+    "hsidm_scale_tensors": [C.POINTER(TensorItem), _i32, _vp, _vp],
 }
-RESTYPE_I64 = {"hsidm_conv_wgrad_workspace_bytes", "hsidm_conv_workspace_bytes"}
+RESTYPE_I64 = {"hsidm_grad_norm_workspace_bytes", "hsidm_conv_wgrad_workspace_bytes", "hsidm_conv_workspace_bytes"}
 
 _lib = None
 

@@ -1,0 +1,215 @@
+// Global gradient norm over many tensors, and clipping:
+//   norm = grad_scale * sqrt(sum over all tensors and elements of g^2),   coef = min(1, max_norm / (norm + 1e-6)),   g <- coef * g
+// Bound by HBM: the norm reads every element once.  The tensors' addresses travel as kernel arguments (kItems per launch), so nothing
+// is copied to the device and a captured launch keeps them; every workgroup sums one run of `chunk` elements of one tensor and writes
+// its sum to a slot of its own, and one workgroup adds the slots in a fixed order: the result does not depend on scheduling.
+// Squares and sums are held in 64 bits - a float's square fits, so neither large nor tiny gradients over- or underflow; two 64-bit
+// instructions per element hide behind the loads.
+#include "common.h"
+#include "../../include/hsidm.h"
+
+namespace hsidm {
+
+constexpr int kItems = 128;                  // 128 * (8 + 8 + 4 + 1) bytes of the 4 KB argument block
+constexpr int kTargetBlocks = 2048;          // eight workgroups per CU when the gradients are large enough
+constexpr int64_t kMinChunk = 4096;
+
+struct NormArgs {
+    const void* ptr[kItems];
+    int64_t n[kItems];
+    int32_t first[kItems + 1];               // first workgroup of every tensor; first[count] = the grid
+    uint8_t type[kItems];
+    int32_t count;
+    int32_t slot0;                           // this launch's first partial sum
+    int64_t chunk;                           // elements per workgroup
+};
+
+// the tensor a workgroup works on, and its run of elements [lo, hi) there (uniform over the workgroup)
+__device__ __forceinline__ void norm_run(const NormArgs& a, int& item, int64_t& lo, int64_t& hi) {
+    int l = 0, r = a.count - 1;
+    while (l < r) {
+        const int m = (l + r + 1) >> 1;
+        if (a.first[m] <= (int)blockIdx.x) l = m; else r = m - 1;
+    }
+    item = l;
+    lo = (int64_t)((int)blockIdx.x - a.first[l]) * a.chunk;
+    hi = lo + a.chunk < a.n[l] ? lo + a.chunk : a.n[l];
+}
+
+// elements of a run ahead of its first 16-byte boundary (views may start anywhere)
+template <typename T> __device__ __forceinline__ int64_t head_of(const T* p, int64_t n) {
+    const int64_t h = ((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T);
+    return h < n ? h : n;
+}
+
+template <typename T> struct Vec16;           // 16 bytes of elements
+template <> struct Vec16<float> { typedef f32x4 type; };
+template <> struct Vec16<bf16> { typedef bf16x8 type; };
+template <> struct Vec16<f16> { typedef f16x8 type; };
+
+template <typename T>
+__device__ __forceinline__ double run_square_sum(const T* p, int64_t n) {
+    typedef typename Vec16<T>::type V;
+    constexpr int E = 16 / sizeof(T);
+    double s = 0.0;
+    const int64_t h = head_of(p, n);
+    if ((int64_t)threadIdx.x < h) { const double x = (double)(float)p[threadIdx.x]; s = x * x; }
+    const int64_t nv = (n - h) / E;
+    const V* q = reinterpret_cast<const V*>(p + h);
+    auto add = [&](const V& v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) { const double x = (double)(float)v[k]; s = fma(x, x, s); }
+    };
+    int64_t i = threadIdx.x;
+    for (; i + 3 * 256 < nv; i += 4 * 256) {  // four loads in flight
+        const V a = q[i], b = q[i + 256], c = q[i + 512], d = q[i + 768];
+        add(a); add(b); add(c); add(d);
+    }
+    for (; i < nv; i += 256) add(q[i]);
+    const int64_t t = h + nv * E + threadIdx.x;
+    if (t < n) { const double x = (double)(float)p[t]; s = fma(x, x, s); }
+    return s;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) v += lds[w];
+    return v;
+}
+
+__global__ __launch_bounds__(256) void norm_partial_kernel(NormArgs a, double* __restrict__ part) {
+    __shared__ double lds[4];
+    int item;
+    int64_t lo, hi;
+    norm_run(a, item, lo, hi);
+    double s;
+    if (a.type[item] == HSIDM_BF16) s = run_square_sum(reinterpret_cast<const bf16*>(a.ptr[item]) + lo, hi - lo);
+    else if (a.type[item] == HSIDM_F16) s = run_square_sum(reinterpret_cast<const f16*>(a.ptr[item]) + lo, hi - lo);
+    else s = run_square_sum(reinterpret_cast<const float*>(a.ptr[item]) + lo, hi - lo);
+    s = block_sum(s, lds);
+    if (threadIdx.x == 0) part[a.slot0 + blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(256) void norm_finish_kernel(const double* __restrict__ part, int nparts, double grad_scale, double max_norm,
+                                                          float* __restrict__ out2) {
+    __shared__ double lds[4];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < nparts; i += 256) s += part[i];
+    s = block_sum(s, lds);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(s) * grad_scale;
+        const double c = max_norm / (norm + 1e-6);
+        out2[0] = (float)norm;
+        out2[1] = max_norm > 1.7e308 ? 1.0f : (c > 1.0 ? 1.0f : (float)c);        // a NaN norm gives a NaN coefficient
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void run_scale(T* p, int64_t n, float c) {
+    typedef typename Vec16<T>::type V;
+    constexpr int E = 16 / sizeof(T);
+    const int64_t h = head_of(p, n);
+    if ((int64_t)threadIdx.x < h) p[threadIdx.x] = (T)((float)p[threadIdx.x] * c);
+    const int64_t nv = (n - h) / E;
+    V* q = reinterpret_cast<V*>(p + h);
+    for (int64_t i = threadIdx.x; i < nv; i += 256) {
+        V v = q[i];
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = (T)((float)v[k] * c);
+        q[i] = v;
+    }
+    const int64_t t = h + nv * E + threadIdx.x;
+    if (t < n) p[t] = (T)((float)p[t] * c);
+}
+
+// (a coefficient of one leaves every element what it is: the launch ends there)
+__global__ __launch_bounds__(256) void norm_scale_kernel(NormArgs a, const float* __restrict__ coef) {
+    const float c = coef[0];
+    if (c == 1.0f) return;
+    int item;
+    int64_t lo, hi;
+    norm_run(a, item, lo, hi);
+    if (a.type[item] == HSIDM_BF16) run_scale(reinterpret_cast<bf16*>(const_cast<void*>(a.ptr[item])) + lo, hi - lo, c);
+    else if (a.type[item] == HSIDM_F16) run_scale(reinterpret_cast<f16*>(const_cast<void*>(a.ptr[item])) + lo, hi - lo, c);
+    else run_scale(reinterpret_cast<float*>(const_cast<void*>(a.ptr[item])) + lo, hi - lo, c);
+}
+
+// Fills the argument block with the tensors from `at` on (empty ones take no workgroup); returns the next tensor.
+static int fill_args(const hsidm_tensor_item* items, int n, int at, int64_t chunk, NormArgs& a) {
+    a.count = 0;
+    a.chunk = chunk;
+    int64_t blocks = 0;
+    for (; at < n && a.count < kItems; ++at) {
+        if (items[at].n == 0) continue;
+        const int k = a.count++;
+        a.ptr[k] = items[at].ptr; a.n[k] = items[at].n; a.type[k] = (uint8_t)items[at].type; a.first[k] = (int32_t)blocks;
+        blocks += (items[at].n + chunk - 1) / chunk;
+    }
+    a.first[a.count] = (int32_t)blocks;
+    return at;
+}
+
+static int check_items(const hsidm_tensor_item* items, int n, int64_t* total) {
+    if (n < 0 || (n > 0 && !items)) return HSIDM_E_BADARG;
+    *total = 0;
+    for (int i = 0; i < n; ++i) {
+        const int t = items[i].type, es = t == HSIDM_F32X3 ? 4 : 2;
+        if (t != HSIDM_BF16 && t != HSIDM_F16 && t != HSIDM_F32X3) return HSIDM_E_BADARG;
+        if (items[i].n < 0 || items[i].n > ((int64_t)1 << 46) || (items[i].n > 0 && (!items[i].ptr || (uintptr_t)items[i].ptr % es))) return HSIDM_E_BADARG;
+        *total += items[i].n;
+        if (*total > ((int64_t)1 << 46)) return HSIDM_E_BADARG;
+    }
+    return 0;
+}
+
+// elements per workgroup: about kTargetBlocks workgroups over all tensors, whole 4096s (the 16-byte alignment of a run is its tensor's)
+static int64_t chunk_of(int64_t total) { return (total / kTargetBlocks + kMinChunk - 1) / kMinChunk * kMinChunk + (total < kTargetBlocks ? kMinChunk : 0); }
+
+}  // namespace hsidm
+
+using namespace hsidm;
+
+extern "C" int64_t hsidm_grad_norm_workspace_bytes(int n_items) {
+    if (n_items < 0) return HSIDM_E_BADARG;
+    return ((int64_t)kTargetBlocks + n_items + 1) * (int64_t)sizeof(double);
+}
+
+extern "C" int hsidm_grad_norm(const hsidm_tensor_item* host_items, int n_items, double grad_scale, double max_norm, void* workspace, float* out2,
+                               void* stream) {
+    int64_t total;
+    if (int rc = check_items(host_items, n_items, &total)) return rc;
+    if (!workspace || !out2 || !(max_norm > 0.0) || !(grad_scale > 0.0)) return HSIDM_E_BADARG;
+    hipStream_t s = (hipStream_t)stream;
+    const int64_t chunk = chunk_of(total);
+    double* part = (double*)workspace;
+    int slots = 0;
+    for (int at = 0; at < n_items;) {
+        NormArgs a;
+        at = fill_args(host_items, n_items, at, chunk, a);
+        if (a.count == 0) break;
+        a.slot0 = slots;
+        hipLaunchKernelGGL(norm_partial_kernel, dim3(a.first[a.count]), dim3(256), 0, s, a, part);
+        slots += a.first[a.count];
+    }
+    hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(256), 0, s, (const double*)part, slots, grad_scale, max_norm, out2);
+    return (int)hipGetLastError();
+}
+
+extern "C" int hsidm_scale_tensors(const hsidm_tensor_item* host_items, int n_items, const float* coef, void* stream) {
+    int64_t total;
+    if (int rc = check_items(host_items, n_items, &total)) return rc;
+    if (!coef) return HSIDM_E_BADARG;
+    const int64_t chunk = chunk_of(total);
+    for (int at = 0; at < n_items;) {
+        NormArgs a;
+        at = fill_args(host_items, n_items, at, chunk, a);
+        if (a.count == 0) break;
+        a.slot0 = 0;
+        hipLaunchKernelGGL(norm_scale_kernel, dim3(a.first[a.count]), dim3(256), 0, (hipStream_t)stream, a, coef);
+    }
+    return (int)hipGetLastError();
+}

@@ -473,7 +473,9 @@ __global__ __launch_bounds__(256) void noise_mlp_bwd_kernel(const float* __restr
 // ---- Adam (torch.optim.Adam, no weight decay / amsgrad; model/model.py:37-41) -------------------------------------------------
 __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
                                                    float* __restrict__ v, int64_t n, float beta1, float beta2, float step_size,
-                                                   float inv_sqrt_bc2, float eps, float grad_scale, const float* __restrict__ coef) {
+                                                   float inv_sqrt_bc2, float eps, float grad_scale, const float* __restrict__ coef,
+                                                   const float* __restrict__ clip) {
+    if (clip) grad_scale *= clip[0];                                // hsidm_grad_norm's coefficient: the clipped gradient is never written
     if (coef) { step_size = coef[0]; inv_sqrt_bc2 = coef[1]; }      // a captured step: the bias corrections come from device memory
     const int64_t n4 = n >> 2;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
@@ -676,12 +678,17 @@ extern "C" int hsidm_gather_pack(const float* src, const int32_t* idx, int64_t n
     return (int)hipGetLastError();
 }
 
-extern "C" int hsidm_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
-                               int step, float grad_scale, const float* coef_dev, void* stream) {
+extern "C" int hsidm_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
+                                       int step, float grad_scale, const float* coef_dev, const float* clip_dev, void* stream) {
     if (!p || !g || !m || !v || n <= 0 || (step <= 0 && !coef_dev)) return HSIDM_E_BADARG;
     const int st = step > 0 ? step : 1;
     const double bc1 = 1.0 - pow((double)beta1, st), bc2 = 1.0 - pow((double)beta2, st);
     hipLaunchKernelGGL(adam_kernel, dim3(grid_for((n + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p, g, m, v, n, beta1, beta2,
-                       (float)((double)lr / bc1), (float)(1.0 / sqrt(bc2)), eps, grad_scale, coef_dev);
+                       (float)((double)lr / bc1), (float)(1.0 / sqrt(bc2)), eps, grad_scale, coef_dev, clip_dev);
     return (int)hipGetLastError();
+}
+
+extern "C" int hsidm_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
+                               int step, float grad_scale, const float* coef_dev, void* stream) {
+    return hsidm_adam_step_clipped(p, g, m, v, n, lr, beta1, beta2, eps, step, grad_scale, coef_dev, nullptr, stream);
 }

@@ -1,6 +1,7 @@
 """Host-side wrappers of the training kernels (include/hsidm.h, "training step"): NHWC tensors of the mode's storage type in,
 kernels enqueued on the current stream, nothing synchronised.  Forward convolutions and their input gradients go through
 ops.conv2d (the input gradient of a convolution is a convolution with the transposed, flipped weights)."""
+import contextlib
 import ctypes as C
 
 import torch
@@ -269,7 +270,105 @@ def adam_coefs(lr, beta1, beta2, step):
     return float(lr / (1.0 - beta1 ** step)), float(1.0 / (1.0 - beta2 ** step) ** 0.5)
 
 
-def adam_step(p, g, m, v, lr, beta1, beta2, eps, step, grad_scale=1.0, coef=None):
-    """coef: optional device tensor of two floats (adam_coefs) read by the kernel instead of deriving them from `step`."""
-    _check(_lib.lib().hsidm_adam_step(_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), _lib.ptr(v), p.numel(), float(lr), float(beta1), float(beta2),
-                                      float(eps), int(step), float(grad_scale), _lib.ptr(coef), _lib.stream_ptr()), "adam_step")
+def adam_step(p, g, m, v, lr, beta1, beta2, eps, step, grad_scale=1.0, coef=None, clip=None):
+    """coef: optional device tensor of two floats (adam_coefs) read by the kernel instead of deriving them from `step`.
+    clip: optional result of clip_coef: the gradient enters scaled by its coefficient (and is not rewritten)."""
+    args = (_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), _lib.ptr(v), p.numel(), float(lr), float(beta1), float(beta2), float(eps), int(step),
+            float(grad_scale), _lib.ptr(coef))
+    if clip is None:
+        _check(_lib.lib().hsidm_adam_step(*args, _lib.stream_ptr()), "adam_step")
+        return
+    if clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or clip.device != p.device:
+        raise ValueError("hsidm: clip must be clip_coef's fp32 [2] on the parameters' device")
+    _check(_lib.lib().hsidm_adam_step_clipped(*args, _lib.ptr(clip) + 4, _lib.stream_ptr()), "adam_step")
+
+
+# ------------------------------------------------------------------------------------------------ global gradient norm and clipping
+_ITEM_TYPE = {torch.float32: _lib.F32X3, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _is_dense(t):
+    """Does the tensor occupy numel() consecutive elements (in any order of its axes)?"""
+    n = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+class TensorList:
+    """The tensors of a gradient norm or clipping call, checked once: dense fp32 / bf16 / fp16 ROCm tensors of one device, mixed types
+    as they come (None entries - parameters without a gradient - are left out).  A program that keeps its gradient tensors keeps the
+    list too; addresses and sizes are read again on every call, so tensors that were given new storage are followed."""
+
+    def __init__(self, tensors):
+        tensors = [tensors] if torch.is_tensor(tensors) else [t for t in tensors if t is not None]
+        for t in tensors:
+            if not torch.is_tensor(t) or t.layout != torch.strided:
+                raise TypeError("hsidm: gradients must be strided tensors, got %s" % type(t).__name__)
+            if not t.is_cuda:
+                raise RuntimeError("hsidm: tensor is on %s; the HIP path needs a ROCm device tensor" % t.device)
+        if len({t.device for t in tensors}) > 1:
+            raise ValueError("hsidm: the tensors of one gradient norm must be on one device")
+        self.tensors = tensors
+        self.device = tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
+        self._key, self._items, self._disjoint = None, None, None
+
+    def items(self):
+        key = [(t.data_ptr(), t.shape, t.stride(), t.dtype) for t in self.tensors]
+        if key != self._key:
+            arr = (_lib.TensorItem * max(1, len(self.tensors)))()
+            for it, t in zip(arr, self.tensors):
+                if t.dtype not in _ITEM_TYPE:
+                    raise TypeError("hsidm: gradients must be fp32, bf16 or fp16, got %s" % t.dtype)
+                if t.numel() and not _is_dense(t):
+                    raise ValueError("hsidm: a gradient of shape %s with strides %s is not dense" % (tuple(t.shape), t.stride()))
+                it.ptr, it.n, it.type = t.data_ptr(), t.numel(), _ITEM_TYPE[t.dtype]
+            spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.tensors if t.numel())
+            self._disjoint = all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+            self._items, self._key = arr, key
+        return self._items
+
+    def disjoint(self):
+        self.items()
+        return self._disjoint
+
+
+def _on(device):
+    """Makes a device current for the launches inside (they go to ITS current stream)."""
+    return contextlib.nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+
+
+def clip_coef(tensors, max_norm, grad_scale=1.0):
+    """fp32 device tensor (norm, coefficient): norm = grad_scale * the 2-norm over all elements of all tensors, coefficient =
+    min(1, max_norm / (norm + 1e-6)) (torch.nn.utils.clip_grad_norm_'s); nothing is synchronised.  tensors: a TensorList, a tensor or
+    an iterable of tensors.  adam_step(clip=...) takes the result."""
+    tl = tensors if isinstance(tensors, TensorList) else TensorList(tensors)
+    if not float(max_norm) > 0 or not 0 < float(grad_scale) < float("inf"):
+        raise ValueError("hsidm: max_norm and grad_scale must be positive, got %r and %r" % (max_norm, grad_scale))
+    L, n, items = _lib.lib(), len(tl.tensors), tl.items()
+    with _on(tl.device):
+        ws = torch.empty(L.hsidm_grad_norm_workspace_bytes(n) // 8, dtype=torch.float64, device=tl.device)
+        out = torch.empty(2, dtype=torch.float32, device=tl.device)
+        _check(L.hsidm_grad_norm(items, n, float(grad_scale), float(max_norm), _lib.ptr(ws), _lib.ptr(out), _lib.stream_ptr()), "grad_norm")
+    return out
+
+
+def grad_norm(tensors, grad_scale=1.0):
+    """The global 2-norm of a list of gradients (times grad_scale) as a 0-dim fp32 device tensor."""
+    return clip_coef(tensors, float("inf"), grad_scale)[0]
+
+
+def clip_grad_norm_(tensors, max_norm):
+    """Scales the tensors in place so that their global 2-norm is at most max_norm; returns the norm from before as a 0-dim fp32 device
+    tensor (torch.nn.utils.clip_grad_norm_ over gradients).  The tensors must not overlap (a shared one would be scaled twice)."""
+    tl = tensors if isinstance(tensors, TensorList) else TensorList(tensors)
+    if not tl.disjoint():
+        raise ValueError("hsidm: clip_grad_norm_ needs tensors that do not overlap (is one of them listed twice?)")
+    out = clip_coef(tl, max_norm)
+    with _on(tl.device):
+        _check(_lib.lib().hsidm_scale_tensors(tl.items(), len(tl.tensors), _lib.ptr(out) + 4, _lib.stream_ptr()), "scale_tensors")
+    if tl.tensors:
+        torch.autograd.graph.increment_version(tl.tensors)      # written through raw pointers
+    return out[0]

@@ -36,7 +36,9 @@ _NOTICE_DONE = False
 
 
 class Trainer:
-    def __init__(self, gd, lr=1e-5, betas=(0.9, 0.999), eps=1e-8, precision=None, dropout_seed=0, bucket_bytes=64 << 20):
+    def __init__(self, gd, lr=1e-5, betas=(0.9, 0.999), eps=1e-8, precision=None, dropout_seed=0, bucket_bytes=64 << 20, max_grad_norm=None):
+        """max_grad_norm: clip the gradient's global 2-norm to this before Adam (None, as the reference: no clipping); the norm of the
+        last step is left in ``last_grad_norm``."""
         net = gd.denoise_fn
         if not isinstance(net, UNet):
             raise TypeError("hsidm: Trainer needs a GaussianDiffusion over hsi_dmgasr_amd's UNet")
@@ -64,6 +66,8 @@ class Trainer:
                 _NOTICE_DONE = True
             self.precision = "fp32"
         self.lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
+        self._g = None
+        self.max_grad_norm, self.last_grad_norm = max_grad_norm, None
         self.dropout_seed = int(dropout_seed)
         self.bucket_bytes = int(bucket_bytes)
         self.step_count = 0            # optimiser steps taken (Adam's bias correction)
@@ -79,6 +83,17 @@ class Trainer:
         self._flatten()
         self._build_pack_maps()
         self.repack()
+
+    @property
+    def max_grad_norm(self):
+        return self._max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, value):
+        if value is not None and not float(value) > 0:
+            raise ValueError("hsidm: max_grad_norm must be positive or None, got %r" % (value,))
+        self._max_grad_norm = None if value is None else float(value)
+        self._g = None                                 # a captured step has the bound baked in: the next call captures again
 
     def _check_device(self):
         if self.dev.type != "cuda":
@@ -550,6 +565,14 @@ class Trainer:
                 p.grad = self._gview[id(p)]
         return loss * scale
 
+    def _clip(self, grad_scale):
+        """adam_step's clipping argument (the flat gradient buffer's padding is zero and does not count)."""
+        if self._max_grad_norm is None:
+            return {}
+        clip = T.clip_coef(self.grad, self._max_grad_norm, grad_scale)
+        self.last_grad_norm = clip[0]
+        return {"clip": clip}
+
     @torch.no_grad()
     def optimizer_step(self):
         """Adam over the flat buffers (after averaging the gradients over the ranks of the default process group), then
@@ -560,7 +583,8 @@ class Trainer:
             parallel.allreduce_grads_(self.grad, self.bucket_bytes)
         self._reduced = False
         self.step_count += 1
-        T.adam_step(self.flat, self.grad, self.m, self.v, self.lr, self.betas[0], self.betas[1], self.eps, self.step_count, 1.0 / world)
+        T.adam_step(self.flat, self.grad, self.m, self.v, self.lr, self.betas[0], self.betas[1], self.eps, self.step_count, 1.0 / world,
+                    **self._clip(1.0 / world))
         # the kernel wrote through raw pointers: tell torch (and the inference path's packed-weight caches, which key on it)
         torch.autograd.graph.increment_version(self._params)
         self.repack()
@@ -730,6 +754,8 @@ class Trainer:
         g["graph"].replay()
         torch.autograd.graph.increment_version(self._params)    # the replay rewrote the parameters through raw pointers
         self._packed_at = self._versions()
+        if g["norm"] is not None:
+            self.last_grad_norm = g["norm"].clone()
         return g["loss"].clone()                                # (the graph's own tensor is overwritten by the next replay)
 
     def _captured_body(self, g):
@@ -744,6 +770,8 @@ class Trainer:
         scale = 1.0 / float(b * c * h * w)
         loss = ops.loss_sum(noise, eps, gd.loss_type) * scale
         self.backward(T.loss_grad(noise, eps, gd.loss_type, scale, self.precision))
-        T.adam_step(self.flat, self.grad, self.m, self.v, self.lr, self.betas[0], self.betas[1], self.eps, 0, 1.0, coef=g["coef"])
+        T.adam_step(self.flat, self.grad, self.m, self.v, self.lr, self.betas[0], self.betas[1], self.eps, 0, 1.0, coef=g["coef"],
+                    **self._clip(1.0))
+        g["norm"] = self.last_grad_norm if self._max_grad_norm is not None else None
         T.gather_pack(self.flat, self._pack_idx, self._pack_hi, self._pack_lo)
         return loss

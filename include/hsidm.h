@@ -50,7 +50,8 @@ extern "C" {
 #define HSIDM_ACT_NONE  0
 #define HSIDM_ACT_LEAKY 1        /* LeakyReLU(0.01)                                                  */
 
-/* ABI version of this header: bumped whenever a struct below grows, a prototype changes or an entry point is added (2: hsidm_conv_desc
+/* ABI version of this header: bumped whenever a struct below grows or a prototype changes (a new entry point alone does not move it: a
+ * library without it fails to resolve the symbol) (2: hsidm_conv_desc
  * gained w_v2_ls / w_v2_li; 3: hsidm_conv1x1_pair, and the bn == 64 projection steps of w_v2 are padded to three).  hsidm_version() returns the version the LIBRARY was built against; a caller built against another header must refuse
  * to run (a shorter hsidm_conv_desc would be read 16 bytes past its end) - the ctypes binding does (hsi-dmgasr_amd/_lib.py). */
 #define HSIDM_ABI_VERSION 3
@@ -423,6 +424,28 @@ int hsidm_gather_pack(const float* src, const int32_t* idx, int64_t n, void* out
  * device address (two floats) instead of being derived from `step` (captured steps). */
 int hsidm_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
                     int step, float grad_scale, const float* coef_dev, void* stream);
+/* hsidm_adam_step with the gradient further scaled by *clip_dev (hsidm_grad_norm's out2 + 1): clipping without a pass over the
+ * gradients of its own.  clip_dev NULL: hsidm_adam_step. */
+int hsidm_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
+                            int step, float grad_scale, const float* coef_dev, const float* clip_dev, void* stream);
+
+/* ---- global gradient norm and clipping (torch.nn.utils.clip_grad_norm_'s definition, 2-norm) -------------------------------
+ * host_items (HOST memory, read before the call returns): n_items tensors of n elements each, dense, at their element's natural
+ * alignment; type HSIDM_F32X3 (fp32), HSIDM_BF16 or HSIDM_F16, mixed as they come; n == 0 items are skipped.
+ *   out2[0] = norm = grad_scale * sqrt(sum of squares over all items), out2[1] = min(1, max_norm / (norm + 1e-6)); max_norm may be
+ *   infinite (the coefficient is then 1).  Sums in 64 bits, fixed order.  An infinite norm gives 0, a NaN one NaN.
+ * hsidm_scale_tensors multiplies every element of the items by *coef in place (one rounding to the item's type); no two items may
+ *   overlap.  coef == 1: nothing is written.
+ * workspace: hsidm_grad_norm_workspace_bytes(n_items) bytes, 8-byte aligned. */
+typedef struct hsidm_tensor_item {
+    const void* ptr;
+    int64_t n;
+    int32_t type, reserved;
+} hsidm_tensor_item;
+int64_t hsidm_grad_norm_workspace_bytes(int n_items);
+int hsidm_grad_norm(const hsidm_tensor_item* host_items, int n_items, double grad_scale, double max_norm, void* workspace, float* out2,
+                    void* stream);
+int hsidm_scale_tensors(const hsidm_tensor_item* host_items, int n_items, const float* coef, void* stream);
 
 #ifdef __cplusplus
 }
