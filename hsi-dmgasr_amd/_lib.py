@@ -3,6 +3,7 @@
 The library is the product: there is no CPU or eager-PyTorch fallback.  If it cannot be loaded,
 or a tensor is not on a ROCm device, the call raises.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -43,6 +44,12 @@ class TensorItem(C.Structure):
     _fields_ = [("ptr", _vp), ("n", _i64), ("type", _i32), ("reserved", _i32)]
 
 
+class RopeDesc(C.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("q_ts", _i64), ("q_hs", _i64), ("k_ts", _i64), ("k_hs", _i64), ("wq", _vp), ("wk", _vp), ("pos", _vp),
+                ("freq", _vp), ("T", _i64), ("Hq", _i32), ("Hk", _i32), ("D", _i32), ("axes", _i32), ("sections", _i32 * 4), ("prec", _i32),
+                ("eps", _f32)]
+
+
 # name -> argtypes, exactly the prototypes of include/hsidm.h
 SIGNATURES = {
     "hsidm_version": [],
@@ -59,6 +66,9 @@ SIGNATURES = {
     "hsidm_noise_film": [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp],
     "hsidm_film_affine": [_i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp],
     "hsidm_attention": [_i32, _vp, _vp, _i32, _i32, _i32, _vp],
+    "hsidm_qk_norm_rope": [C.POINTER(RopeDesc), _vp, _vp, _vp],
+    "hsidm_qk_norm_rope_bwd_workspace_bytes": [C.POINTER(RopeDesc)],
+    "hsidm_qk_norm_rope_bwd": [C.POINTER(RopeDesc), _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
     "hsidm_nchw_to_nhwc": [_i32, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp],
     "hsidm_nhwc_to_nchw": [_i32, _vp, _vp, _i32, _i32, _i32, _vp],
     "hsidm_p_sample_update": [_vp, _vp, _vp, _vp, _i32, _vp, _i64, _u64, _i64, _vp, _i32, _vp],
@@ -107,7 +117,7 @@ SIGNATURES = {
     "hsidm_grad_norm": [C.POINTER(TensorItem), _i32, _f64, _f64, _vp, _vp, _vp],
     "hsidm_scale_tensors": [C.POINTER(TensorItem), _i32, _vp, _vp],
 }
-RESTYPE_I64 = {"hsidm_grad_norm_workspace_bytes", "hsidm_conv_wgrad_workspace_bytes", "hsidm_conv_workspace_bytes"}
+RESTYPE_I64 = {"hsidm_grad_norm_workspace_bytes", "hsidm_qk_norm_rope_bwd_workspace_bytes", "hsidm_conv_wgrad_workspace_bytes", "hsidm_conv_workspace_bytes"}
 
 _lib = None
 
@@ -171,6 +181,21 @@ def ptr(t):
     if not t.is_contiguous():
         raise RuntimeError("hsidm: tensor must be contiguous")
     return t.data_ptr()
+
+
+_TYPE_ID = {torch.bfloat16: BF16, torch.float32: F32X3, torch.float16: F16}
+
+
+def type_id(dtype):
+    """Element type code of a token-tensor operator (hsidm_qk_norm_rope, hsidm_attention_packed, hsidm_grad_norm)."""
+    if dtype not in _TYPE_ID:
+        raise TypeError("hsidm: tensors must be fp32, bf16 or fp16, got %s" % dtype)
+    return _TYPE_ID[dtype]
+
+
+def on_device(device):
+    """Context in which `device` is current: launches inside go to ITS current stream."""
+    return contextlib.nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
 
 
 def prec_id(precision):

@@ -5,6 +5,7 @@ the storage type of the precision mode (bf16 / fp32), fp32 everywhere else.  tor
 device memory and the current stream.
 """
 import ctypes as C
+import math
 
 import torch
 
@@ -558,6 +559,96 @@ def attention_multihead(qkv, n_head, precision):
         _lib.check(L.hsidm_softmax_rows(_lib.ptr(P), B * N, N, st), "softmax_rows")
         _lib.check(L.hsidm_bgemm(P.data_ptr(), 1, N * N, N, 1, v, int(f32), N * C3, C3, 1, o, int(f32), N * Cc, Cc, N, hd, N, B, 1.0, st), "bgemm")
     return out
+
+
+# ------------------------------------------------------------------------------------------------ token operators
+# [T, heads, D] tensors of packed tokens (fp32, bf16 or fp16), last axis contiguous; views of one projection's output as they come.
+def base(t):
+    """Device pointer of a strided token tensor (refuses host tensors)."""
+    if not t.is_cuda:
+        raise RuntimeError("hsidm: tensor is on %s; the HIP path needs a ROCm device tensor" % t.device)
+    return t.data_ptr()
+
+
+def rows_aligned(t):
+    """Does every (token, head) row of [T, H, D] start on a 16-byte boundary, contiguous along D?"""
+    es = t.element_size()
+    return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] <= 1 or (t.stride(i) * es) % 16 == 0 and t.stride(i) > 0 for i in (0, 1))
+
+
+def token_rows(t):
+    """t itself where the kernels can address its rows, else a contiguous copy (odd offsets or strides, a transposed last axis)."""
+    return t if rows_aligned(t) else t.contiguous() if t.data_ptr() % 16 == 0 or not t.is_contiguous() else t.clone()
+
+
+def _strides(t):
+    """(token, head) strides in elements; an axis of length one has whatever stride torch says: zero serves."""
+    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
+
+
+class RotaryAxes:
+    """Frequencies of a rotary embedding over several position axes (time or band group, row, column): sections[a] pairs of every head turn
+    with axis a, pair j of them by base^(-j / sections[a]) radians per position; pairs beyond sum(sections) (at most D/2) are not turned.
+    Pair p of a head is its elements (p, p + D/2).  The table is built once, in 64 bits."""
+
+    def __init__(self, sections, head_dim, base=10000.0, device="cuda"):
+        self.sections = tuple(int(n) for n in sections)
+        self.head_dim = int(head_dim)
+        if not 1 <= len(self.sections) <= 4 or min(self.sections) < 0:
+            raise ValueError("hsidm: one to four axes with non-negative sections, got %r" % (sections,))
+        if self.head_dim % 16 or not 16 <= self.head_dim <= 256 or sum(self.sections) > self.head_dim // 2:
+            raise ValueError("hsidm: head_dim must be a multiple of 16 up to 256 with at least 2 * %d elements, got %d" % (sum(self.sections), self.head_dim))
+        if not 1.0 < float(base) < float("inf"):
+            raise ValueError("hsidm: base must be greater than one, got %r" % (base,))
+        turns = [float(base) ** (-j / n) / (2.0 * math.pi) for n in self.sections for j in range(n)]
+        self.freq = torch.tensor(turns or [0.0], dtype=torch.float64).to(device)
+
+
+def rope_desc(q, k, wq, wk, pos, axes, eps):
+    """(descriptor, tensors it points into) of hsidm_qk_norm_rope after checking every argument."""
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[1] < 1 or k.shape[1] < 1:
+        raise ValueError("hsidm: q and k must be [T, heads, D] over the same tokens, got %s and %s" % (tuple(q.shape), tuple(k.shape)))
+    T, Hq, D = q.shape
+    if D != axes.head_dim:
+        raise ValueError("hsidm: the heads have %d elements, the axes were built for %d" % (D, axes.head_dim))
+    if q.dtype != k.dtype:
+        raise TypeError("hsidm: q and k must have one type, got %s and %s" % (q.dtype, k.dtype))
+    tid = _lib.type_id(q.dtype)
+    for w in (wq, wk):
+        if w.dtype != torch.float32 or tuple(w.shape) != (D,):
+            raise ValueError("hsidm: norm weights must be fp32 [%d], got %s %s" % (D, w.dtype, tuple(w.shape)))
+    if pos.dtype != torch.int32 or tuple(pos.shape) != (T, len(axes.sections)):
+        raise ValueError("hsidm: positions must be int32 [%d, %d], got %s %s" % (T, len(axes.sections), pos.dtype, tuple(pos.shape)))
+    if any(t.device != q.device for t in (k, wq, wk, pos, axes.freq)):
+        raise ValueError("hsidm: q, k, weights, positions and axes must be on one device")
+    if not float(eps) >= 0:
+        raise ValueError("hsidm: eps must not be negative, got %r" % (eps,))
+    base(q)
+    q, k, wq, wk, pos = token_rows(q), token_rows(k), _aligned(wq), _aligned(wk), pos.contiguous()
+    d = _lib.RopeDesc()
+    d.q, d.k, d.wq, d.wk, d.pos, d.freq = (t.data_ptr() for t in (q, k, wq, wk, pos, axes.freq))
+    (d.q_ts, d.q_hs), (d.k_ts, d.k_hs) = _strides(q), _strides(k)
+    d.T, d.Hq, d.Hk, d.D, d.axes, d.prec, d.eps = T, Hq, k.shape[1], D, len(axes.sections), tid, float(eps)
+    for i, n in enumerate(axes.sections):
+        d.sections[i] = n
+    return d, (q, k, wq, wk, pos)
+
+
+def _aligned(t):
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def qk_norm_rope(q, k, wq, wk, pos, axes, eps=1e-6):
+    """RMS norm of every query and key head (weights wq, wk fp32 [D]) and its rotation by the token's positions, one launch:
+    q [T, Hq, D], k [T, Hk, D] (any strides; rows on 16-byte boundaries are read in place), pos int32 [T, axes], axes a RotaryAxes.
+    -> two contiguous tensors of q's type.  Gradient: train_ops.qk_norm_rope_bwd."""
+    d, keep = rope_desc(q, k, wq, wk, pos, axes, eps)
+    oq, ok = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.shape[0]:
+        with _lib.on_device(q.device):
+            _lib.check(_lib.lib().hsidm_qk_norm_rope(C.byref(d), oq.data_ptr(), ok.data_ptr(), _lib.stream_ptr()), "qk_norm_rope")
+    return oq, ok
 
 
 _offset_cache = {}

@@ -1,7 +1,6 @@
 """Host-side wrappers of the training kernels (include/hsidm.h, "training step"): NHWC tensors of the mode's storage type in,
 kernels enqueued on the current stream, nothing synchronised.  Forward convolutions and their input gradients go through
 ops.conv2d (the input gradient of a convolution is a convolution with the transposed, flipped weights)."""
-import contextlib
 import ctypes as C
 
 import torch
@@ -284,9 +283,6 @@ def adam_step(p, g, m, v, lr, beta1, beta2, eps, step, grad_scale=1.0, coef=None
 
 
 # ------------------------------------------------------------------------------------------------ global gradient norm and clipping
-_ITEM_TYPE = {torch.float32: _lib.F32X3, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
-
-
 def _is_dense(t):
     """Does the tensor occupy numel() consecutive elements (in any order of its axes)?"""
     n = 1
@@ -320,11 +316,9 @@ class TensorList:
         if key != self._key:
             arr = (_lib.TensorItem * max(1, len(self.tensors)))()
             for it, t in zip(arr, self.tensors):
-                if t.dtype not in _ITEM_TYPE:
-                    raise TypeError("hsidm: gradients must be fp32, bf16 or fp16, got %s" % t.dtype)
                 if t.numel() and not _is_dense(t):
                     raise ValueError("hsidm: a gradient of shape %s with strides %s is not dense" % (tuple(t.shape), t.stride()))
-                it.ptr, it.n, it.type = t.data_ptr(), t.numel(), _ITEM_TYPE[t.dtype]
+                it.ptr, it.n, it.type = t.data_ptr(), t.numel(), _lib.type_id(t.dtype)
             spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.tensors if t.numel())
             self._disjoint = all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
             self._items, self._key = arr, key
@@ -335,11 +329,6 @@ class TensorList:
         return self._disjoint
 
 
-def _on(device):
-    """Makes a device current for the launches inside (they go to ITS current stream)."""
-    return contextlib.nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
-
-
 def clip_coef(tensors, max_norm, grad_scale=1.0):
     """fp32 device tensor (norm, coefficient): norm = grad_scale * the 2-norm over all elements of all tensors, coefficient =
     min(1, max_norm / (norm + 1e-6)) (torch.nn.utils.clip_grad_norm_'s); nothing is synchronised.  tensors: a TensorList, a tensor or
@@ -348,7 +337,7 @@ def clip_coef(tensors, max_norm, grad_scale=1.0):
     if not float(max_norm) > 0 or not 0 < float(grad_scale) < float("inf"):
         raise ValueError("hsidm: max_norm and grad_scale must be positive, got %r and %r" % (max_norm, grad_scale))
     L, n, items = _lib.lib(), len(tl.tensors), tl.items()
-    with _on(tl.device):
+    with _lib.on_device(tl.device):
         ws = torch.empty(L.hsidm_grad_norm_workspace_bytes(n) // 8, dtype=torch.float64, device=tl.device)
         out = torch.empty(2, dtype=torch.float32, device=tl.device)
         _check(L.hsidm_grad_norm(items, n, float(grad_scale), float(max_norm), _lib.ptr(ws), _lib.ptr(out), _lib.stream_ptr()), "grad_norm")
@@ -367,8 +356,36 @@ def clip_grad_norm_(tensors, max_norm):
     if not tl.disjoint():
         raise ValueError("hsidm: clip_grad_norm_ needs tensors that do not overlap (is one of them listed twice?)")
     out = clip_coef(tl, max_norm)
-    with _on(tl.device):
+    with _lib.on_device(tl.device):
         _check(_lib.lib().hsidm_scale_tensors(tl.items(), len(tl.tensors), _lib.ptr(out) + 4, _lib.stream_ptr()), "scale_tensors")
     if tl.tensors:
         torch.autograd.graph.increment_version(tl.tensors)      # written through raw pointers
     return out[0]
+
+
+# ------------------------------------------------------------------------------------------------ token operators (ops.qk_norm_rope)
+def qk_norm_rope_bwd(d_out_q, d_out_k, q, k, wq, wk, pos, axes, eps=1e-6, out=None):
+    """Gradient of ops.qk_norm_rope: (dq, dk, dwq, dwk) from the gradients of its two results and its inputs; dq / dk in the inputs'
+    type, dwq / dwk fp32 [D].  out: optional (dq, dk) to write into, [T, H, D] views with 16-byte aligned rows (slices of a dqkv)."""
+    d, keep = ops.rope_desc(q, k, wq, wk, pos, axes, eps)
+    T, D = q.shape[0], q.shape[2]
+    for g, x in ((d_out_q, q), (d_out_k, k)):
+        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
+            raise ValueError("hsidm: a gradient of %s %s does not belong to a tensor of %s %s" % (tuple(g.shape), g.dtype, tuple(x.shape), x.dtype))
+    dq, dk = (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)) if out is None else out
+    for g, x in ((dq, q), (dk, k)):
+        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device or not ops.rows_aligned(g):
+            raise ValueError("hsidm: out must be [T, H, D] tensors like q and k with 16-byte aligned rows")
+    dwq, dwk = (torch.zeros if T == 0 else torch.empty)((2, D), dtype=torch.float32, device=q.device).unbind(0)
+    if T == 0:
+        return dq, dk, dwq, dwk
+    L = _lib.lib()
+    with _lib.on_device(q.device):
+        nb = L.hsidm_qk_norm_rope_bwd_workspace_bytes(C.byref(d))
+        if nb < 0:
+            _check(int(nb), "qk_norm_rope_bwd_workspace_bytes")
+        ws = torch.empty(int(nb), dtype=torch.uint8, device=q.device)
+        gq, gk = d_out_q.contiguous(), d_out_k.contiguous()
+        _check(L.hsidm_qk_norm_rope_bwd(C.byref(d), ops.base(gq), ops.base(gk), ops.base(dq), dq.stride(0), dq.stride(1), ops.base(dk), dk.stride(0),
+                                        dk.stride(1), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), int(nb), _lib.stream_ptr()), "qk_norm_rope_bwd")
+    return dq, dk, dwq, dwk

@@ -219,6 +219,32 @@ int hsidm_film_affine(int prec, const void* x, const float* gamma_beta, void* ou
  */
 int hsidm_attention(int prec, const void* qkv, void* out, int B, int N, int C, void* stream);
 
+/* ---- RMS norm of queries and keys per head + rotation by positions with several axes, one pass -------------------------------
+ * For every token t < T and head of q ([T][Hq][D]) and k ([T][Hk][D]):
+ *   n = x * rsqrt(mean(x^2) + eps) * w (w fp32 [D], one for q and one for k), then pair (n[p], n[p + D/2]), p < P = sum of sections, is
+ *   turned by the angle 2 pi * pos[t][a] * freq[p], a the axis whose section of pairs holds p (axis 0 the first sections[0] pairs, ...);
+ *   the other pairs are left as they are.  freq: turns per position, fp64 [P]; pos int32 [T][axes]; the angle is formed in 64 bits.
+ * D a multiple of 16, 16 ... 256; x's last axis is contiguous, token and head strides in elements (multiples of 16 bytes, 16-byte aligned
+ * bases); fp32, bf16 or fp16 tensors, arithmetic in fp32; out_q / out_k contiguous.
+ * Backward: d_out_q / d_out_k (contiguous) -> dq, dk (strided like x) and dwq, dwk fp32 [D] (sums over tokens and heads in a fixed
+ * order); two launches; workspace: hsidm_qk_norm_rope_bwd_workspace_bytes(desc) bytes. */
+#define HSIDM_ROPE_AXES 4
+typedef struct hsidm_rope_desc {
+    const void *q, *k;
+    int64_t q_ts, q_hs, k_ts, k_hs;          /* token / head strides in elements */
+    const float *wq, *wk;
+    const int32_t* pos;
+    const double* freq;
+    int64_t T;
+    int32_t Hq, Hk, D, axes, sections[HSIDM_ROPE_AXES], prec;
+    float eps;
+} hsidm_rope_desc;
+int hsidm_qk_norm_rope(const hsidm_rope_desc* d, void* out_q, void* out_k, void* stream);
+int64_t hsidm_qk_norm_rope_bwd_workspace_bytes(const hsidm_rope_desc* d);
+int hsidm_qk_norm_rope_bwd(const hsidm_rope_desc* d, const void* d_out_q, const void* d_out_k, void* dq, int64_t dq_ts, int64_t dq_hs,
+                           void* dk, int64_t dk_ts, int64_t dk_hs, float* dwq, float* dwk, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
 /* ---- layout conversion at the reference's module boundaries ----------------------------------------
  * nchw_to_nhwc: out[e][p][c] for c < Cpad (multiple of 8): channel c comes from fp32 NCHW planes
  * src0 + off0[e] + c*HW (c < C0), src1 + off1[e] + (c-C0)*HW (C0 <= c < C0+C1), else 0.
