@@ -50,6 +50,12 @@ class RopeDesc(C.Structure):
                 ("eps", _f32)]
 
 
+class AttnDesc(C.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_ts", _i64), ("q_hs", _i64), ("k_ts", _i64), ("k_hs", _i64), ("v_ts", _i64), ("v_hs", _i64),
+                ("T", _i64), ("qtiles64", _vp), ("qtiles128", _vp), ("ktiles64", _vp), ("ktiles128", _vp), ("n64", _i32), ("n128", _i32),
+                ("longest", _i32), ("Hq", _i32), ("Hk", _i32), ("D", _i32), ("prec", _i32), ("causal", _i32), ("scale", _f32)]
+
+
 # name -> argtypes, exactly the prototypes of include/hsidm.h
 SIGNATURES = {
     "hsidm_version": [],
@@ -66,6 +72,10 @@ SIGNATURES = {
     "hsidm_noise_film": [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp],
     "hsidm_film_affine": [_i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp],
     "hsidm_attention": [_i32, _vp, _vp, _i32, _i32, _i32, _vp],
+    "hsidm_attention_packed_workspace_bytes": [C.POINTER(AttnDesc)],
+    "hsidm_attention_packed": [C.POINTER(AttnDesc), _vp, _vp, _vp, _i64, _vp],
+    "hsidm_attention_packed_bwd_workspace_bytes": [C.POINTER(AttnDesc)],
+    "hsidm_attention_packed_bwd": [C.POINTER(AttnDesc), _vp, _vp] + [_vp, _i64, _i64] * 4 + [_vp, _i64, _vp],
     "hsidm_qk_norm_rope": [C.POINTER(RopeDesc), _vp, _vp, _vp],
     "hsidm_qk_norm_rope_bwd_workspace_bytes": [C.POINTER(RopeDesc)],
     "hsidm_qk_norm_rope_bwd": [C.POINTER(RopeDesc), _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
@@ -117,7 +127,7 @@ SIGNATURES = {
     "hsidm_grad_norm": [C.POINTER(TensorItem), _i32, _f64, _f64, _vp, _vp, _vp],
     "hsidm_scale_tensors": [C.POINTER(TensorItem), _i32, _vp, _vp],
 }
-RESTYPE_I64 = {"hsidm_grad_norm_workspace_bytes", "hsidm_qk_norm_rope_bwd_workspace_bytes", "hsidm_conv_wgrad_workspace_bytes", "hsidm_conv_workspace_bytes"}
+RESTYPE_I64 = {"hsidm_attention_packed_workspace_bytes", "hsidm_attention_packed_bwd_workspace_bytes", "hsidm_grad_norm_workspace_bytes", "hsidm_qk_norm_rope_bwd_workspace_bytes", "hsidm_conv_wgrad_workspace_bytes", "hsidm_conv_workspace_bytes"}
 
 _lib = None
 

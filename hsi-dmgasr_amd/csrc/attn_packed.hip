@@ -1,0 +1,273 @@
+// Attention over packed sequences: the C entry points, the choice of tile and split, and the small kernels around the main ones
+// (attn_packed.h): joining split key ranges, the backward pass's row sums, adding split partial gradients.
+#include "attn_packed.h"
+
+namespace hsidm {
+
+// Joins the shares of a split forward pass: part [S][T][Hq][D] fp32 normalised outputs, plse [S][Hq][T]; a row's weight of share s is
+// exp(lse_s - lse).  Four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, const float* __restrict__ plse, int S, int64_t T_, int Hq, int D,
+                                                        T* __restrict__ out, float* __restrict__ lse) {
+    const int per_row = D / 4;
+    const int64_t n = T_ * Hq * per_row, rows = T_ * Hq;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per_row;
+        const int d = (int)(i - row * per_row) * 4, head = (int)(row % Hq);
+        const int64_t at = head * T_ + row / Hq;
+        float m = -INFINITY;
+        for (int s = 0; s < S; ++s) m = fmaxf(m, plse[s * rows + at]);
+        const float mm = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < S; ++s) {
+            const float w = __expf(plse[s * rows + at] - mm);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(part + (s * rows + row) * D + d);
+            l += w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += w * x[k];
+        }
+        typedef T vec __attribute__((ext_vector_type(4)));
+        vec r;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = (T)(v[k] * inv);
+        *reinterpret_cast<vec*>(out + row * D + d) = r;
+        if (lse && d == 0) lse[at] = mm + logf(l);
+    }
+}
+
+// out[t][h][d] = sum over the shares of part[s * share + (t * H + h) * D + d], in order
+template <typename T>
+__global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__ part, int S, int64_t share, int64_t T_, int H, int D, AttnTensor out) {
+    const int per_row = D / 4;
+    const int64_t n = T_ * H * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per_row, token = row / H;
+        const int d = (int)(i - row * per_row) * 4, head = (int)(row - token * H);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < S; ++s) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(part + s * share + row * D + d);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += x[k];
+        }
+        typedef T vec __attribute__((ext_vector_type(4)));
+        vec r;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = (T)v[k];
+        *reinterpret_cast<vec*>(reinterpret_cast<T*>(const_cast<char*>(out.p) + token * out.ts + head * out.hs) + d) = r;
+    }
+}
+
+// delta[h][t] = sum_d dO O per row; fp16: also this workgroup's largest |dO|^2 and |V|^2 (GradScale).  `group` lanes, a power of two that
+// covers a row's 16-byte pieces, share a row.
+constexpr int kDeltaBlocks = 512;
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTensor o, AttnTensor v, int64_t T_, int Hq, int Hk, int pieces, int group,
+                                                         float* __restrict__ delta, float* __restrict__ maxima) {
+    constexpr int E = 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(E)));
+    __shared__ float red[2][4];
+    const int sub = threadIdx.x & (group - 1), per = 256 / group;
+    auto sum = [&](float x) __attribute__((always_inline)) {
+        for (int s = group >> 1; s > 0; s >>= 1) x += __shfl_xor(x, s, 64);
+        return x;
+    };
+    float ma = 0.f, mb = 0.f;
+    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < T_ * Hq; r0 += (int64_t)gridDim.x * per) {
+        const int64_t r = r0 + threadIdx.x / group, token = r / Hq;
+        const int head = (int)(r - token * Hq);
+        float dot = 0.f, sq = 0.f;
+        if (r < T_ * Hq && sub < pieces) {
+            const vec x = *reinterpret_cast<const vec*>(dout.p + token * dout.ts + head * dout.hs + sub * 16);
+            const vec y = *reinterpret_cast<const vec*>(o.p + token * o.ts + head * o.hs + sub * 16);
+#pragma unroll
+            for (int k = 0; k < E; ++k) { dot += (float)x[k] * (float)y[k]; sq += (float)x[k] * (float)x[k]; }
+        }
+        dot = sum(dot);
+        if (GradScale<T>::on) ma = fmaxf(ma, sum(sq));
+        if (r < T_ * Hq && sub == 0) delta[head * T_ + token] = dot;
+    }
+    if constexpr (GradScale<T>::on) {
+        for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < T_ * Hk; r0 += (int64_t)gridDim.x * per) {
+            const int64_t r = r0 + threadIdx.x / group, token = r / Hk;
+            const int head = (int)(r - token * Hk);
+            float sq = 0.f;
+            if (r < T_ * Hk && sub < pieces) {
+                const vec x = *reinterpret_cast<const vec*>(v.p + token * v.ts + head * v.hs + sub * 16);
+#pragma unroll
+                for (int k = 0; k < E; ++k) sq += (float)x[k] * (float)x[k];
+            }
+            mb = fmaxf(mb, sum(sq));
+        }
+        ma = wave_max(ma); mb = wave_max(mb);
+        if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = ma; red[1][threadIdx.x >> 6] = mb; }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            maxima[2 * blockIdx.x] = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+            maxima[2 * blockIdx.x + 1] = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+        }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+struct Cut { int waves, ntiles, splits; };
+
+// Tile height and split of the long axis.  128-row tiles (4 waves) where they give every CU a workgroup, else 64-row ones.  The walked axis
+// (`steps` tiles of the longest sequence) is split, into shares of at least four tiles, while the waves do not reach two per SIMD.
+static Cut cut_work(int heads, int n64, int n128, int64_t steps) {
+    Cut c;
+    c.waves = (int64_t)n128 * heads >= device_cus() ? 4 : 2;
+    c.ntiles = c.waves == 4 ? n128 : n64;
+    const int64_t waves = (int64_t)c.ntiles * heads * c.waves, want = (int64_t)device_cus() * 8;
+    int64_t s = waves > 0 ? want / waves : 1;
+    if (s > steps / 4) s = steps / 4;
+    if (s > 16) s = 16;
+    c.splits = s > 1 ? (int)s : 1;
+    return c;
+}
+static int tile_rows(int D, int es) { return (D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256) * es <= 256 ? 64 : 32; }
+
+static bool rows_ok(const void* p, int64_t ts, int64_t hs, int es) {
+    return p && (uintptr_t)p % 16 == 0 && ts >= 0 && hs >= 0 && ts * es % 16 == 0 && hs * es % 16 == 0;
+}
+static int check_attn(const hsidm_attn_desc* d, int& es) {
+    if (!d || (d->prec != HSIDM_BF16 && d->prec != HSIDM_F16 && d->prec != HSIDM_F32X3)) return HSIDM_E_BADARG;
+    es = d->prec == HSIDM_F32X3 ? 4 : 2;
+    if (d->T <= 0 || d->T > 0x7fffffff || d->Hk <= 0 || d->Hq <= 0 || d->Hq % d->Hk || d->Hq > 65535) return HSIDM_E_BADARG;
+    if (d->D < 16 / es || d->D > 256 || d->D * es % 16) return HSIDM_E_BADARG;
+    if (!(d->scale > 0.f) || !(d->scale < 1e30f)) return HSIDM_E_BADARG;
+    if (!rows_ok(d->q, d->q_ts, d->q_hs, es) || !rows_ok(d->k, d->k_ts, d->k_hs, es) || !rows_ok(d->v, d->v_ts, d->v_hs, es)) return HSIDM_E_BADARG;
+    if (!d->qtiles64 || !d->qtiles128 || !d->ktiles64 || !d->ktiles128 || d->n64 <= 0 || d->n128 <= 0 || d->longest <= 0) return HSIDM_E_BADARG;
+    if ((int64_t)d->n64 * d->Hq > 0x7fffffff) return HSIDM_E_UNSUPPORTED;
+    return 0;
+}
+static AttnTensor tensor(const void* p, int64_t ts, int64_t hs, int es) { return {(const char*)p, ts * es, hs * es}; }
+static int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+static int launch(int prec, int kind, const void* args, const Cut& c, hipStream_t s) {
+    if (prec == HSIDM_BF16) return attn_launch<bf16>(kind, args, c.waves, c.ntiles, s);
+    if (prec == HSIDM_F16) return attn_launch<f16>(kind, args, c.waves, c.ntiles, s);
+    return attn_launch<float>(kind, args, c.waves, c.ntiles, s);
+}
+static unsigned blocks_for(int64_t n) { const int64_t b = (n + 255) / 256; return (unsigned)(b < 65536 ? b : 65536); }
+
+struct BwdPlan { Cut q, kv; int64_t delta, maxima, part, bytes; int nmax; };
+static BwdPlan bwd_plan(const hsidm_attn_desc* d, int es) {
+    BwdPlan p;
+    const int64_t steps = (d->longest + tile_rows(d->D, es) - 1) / tile_rows(d->D, es);
+    p.q = cut_work(d->Hq, d->n64, d->n128, steps);
+    p.kv = cut_work(d->Hk, d->n64, d->n128, steps * (d->Hq / d->Hk));
+    int group = 1;
+    while (group < d->D * es / 16) group *= 2;
+    const int64_t rows = d->T * d->Hq, blocks = (rows * group + 255) / 256;
+    p.nmax = (int)(blocks < kDeltaBlocks ? blocks : kDeltaBlocks);
+    p.delta = 0;
+    p.maxima = up16(rows * 4);
+    p.part = p.maxima + up16((int64_t)p.nmax * 8);
+    const int64_t pq = p.q.splits > 1 ? (int64_t)p.q.splits * d->T * d->Hq * d->D * 4 : 0;
+    const int64_t pkv = p.kv.splits > 1 ? (int64_t)p.kv.splits * 2 * d->T * d->Hk * d->D * 4 : 0;
+    p.bytes = p.part + (pq > pkv ? pq : pkv);                         // (one after the other on the stream: they share the space)
+    return p;
+}
+
+template <typename T>
+static void launch_delta(const AttnTensor& dout, const AttnTensor& o, const AttnTensor& v, const hsidm_attn_desc* d, int pieces, int nmax, float* delta,
+                         float* maxima, hipStream_t s) {
+    int group = 1;
+    while (group < pieces) group *= 2;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_delta_kernel<T>), dim3(nmax), dim3(256), 0, s, dout, o, v, d->T, d->Hq, d->Hk, pieces, group, delta, maxima);
+}
+template <typename T>
+static void launch_add(const float* part, const Cut& c, int64_t share, int64_t T_, int H, int D, const AttnTensor& out, hipStream_t s) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_add_kernel<T>), dim3(blocks_for(T_ * H * D / 4)), dim3(256), 0, s, part, c.splits, share, T_, H, D, out);
+}
+static void add_parts(int prec, const float* part, const Cut& c, int64_t share, int64_t T_, int H, int D, const AttnTensor& out, hipStream_t s) {
+    if (prec == HSIDM_BF16) launch_add<bf16>(part, c, share, T_, H, D, out, s);
+    else if (prec == HSIDM_F16) launch_add<f16>(part, c, share, T_, H, D, out, s);
+    else launch_add<float>(part, c, share, T_, H, D, out, s);
+}
+
+}  // namespace hsidm
+
+using namespace hsidm;
+
+extern "C" int64_t hsidm_attention_packed_workspace_bytes(const hsidm_attn_desc* d) {
+    int es;
+    if (int rc = check_attn(d, es)) return rc;
+    const Cut c = cut_work(d->Hq, d->n64, d->n128, (d->longest + tile_rows(d->D, es) - 1) / tile_rows(d->D, es));
+    return c.splits > 1 ? (int64_t)c.splits * d->T * d->Hq * (d->D + 1) * 4 : 0;
+}
+
+extern "C" int hsidm_attention_packed(const hsidm_attn_desc* d, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    int es;
+    if (int rc = check_attn(d, es)) return rc;
+    if (!rows_ok(out, 0, 0, es)) return HSIDM_E_BADARG;
+    const Cut c = cut_work(d->Hq, d->n64, d->n128, (d->longest + tile_rows(d->D, es) - 1) / tile_rows(d->D, es));
+    const int64_t rows = d->T * d->Hq;
+    if (c.splits > 1 && (!rows_ok(workspace, 0, 0, 4) || workspace_bytes < c.splits * rows * (d->D + 1) * 4)) return HSIDM_E_BADARG;
+    AttnFwdArgs a;
+    a.q = tensor(d->q, d->q_ts, d->q_hs, es); a.k = tensor(d->k, d->k_ts, d->k_hs, es); a.v = tensor(d->v, d->v_ts, d->v_hs, es);
+    float* part = (float*)workspace;
+    a.out = c.splits > 1 ? (void*)part : out;
+    a.lse = c.splits > 1 ? part + c.splits * rows * d->D : lse;
+    a.tiles = (const AttnTile*)(c.waves == 4 ? d->qtiles128 : d->qtiles64);
+    a.T = d->T; a.Hq = d->Hq; a.Hk = d->Hk; a.D = d->D; a.causal = d->causal; a.splits = c.splits; a.scale = d->scale;
+    hipStream_t s = (hipStream_t)stream;
+    if (int rc = launch(d->prec, ATTN_FWD, &a, c, s)) return rc;
+    if (c.splits > 1) {
+        const dim3 grid(blocks_for(rows * d->D / 4));
+        const float* pl = part + c.splits * rows * d->D;
+#define JOIN(OUT) hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_join_kernel<OUT>), grid, dim3(256), 0, s, (const float*)part, pl, c.splits, d->T, d->Hq, d->D, (OUT*)out, lse)
+        if (d->prec == HSIDM_BF16) JOIN(bf16);
+        else if (d->prec == HSIDM_F16) JOIN(f16);
+        else JOIN(float);
+#undef JOIN
+    }
+    return (int)hipGetLastError();
+}
+
+extern "C" int64_t hsidm_attention_packed_bwd_workspace_bytes(const hsidm_attn_desc* d) {
+    int es;
+    if (int rc = check_attn(d, es)) return rc;
+    return bwd_plan(d, es).bytes;
+}
+
+extern "C" int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* out, const float* lse, const void* dout, int64_t do_ts, int64_t do_hs,
+                                          void* dq, int64_t dq_ts, int64_t dq_hs, void* dk, int64_t dk_ts, int64_t dk_hs, void* dv, int64_t dv_ts,
+                                          int64_t dv_hs, void* workspace, int64_t workspace_bytes, void* stream) {
+    int es;
+    if (int rc = check_attn(d, es)) return rc;
+    if (!lse || !rows_ok(out, 0, 0, es) || !rows_ok(dout, do_ts, do_hs, es) || !rows_ok(dq, dq_ts, dq_hs, es) || !rows_ok(dk, dk_ts, dk_hs, es) ||
+        !rows_ok(dv, dv_ts, dv_hs, es))
+        return HSIDM_E_BADARG;
+    const BwdPlan p = bwd_plan(d, es);
+    if (!rows_ok(workspace, 0, 0, 4) || workspace_bytes < p.bytes) return HSIDM_E_BADARG;
+    char* ws = (char*)workspace;
+    float *delta = (float*)(ws + p.delta), *maxima = (float*)(ws + p.maxima);
+    hipStream_t s = (hipStream_t)stream;
+    AttnBwdArgs a;
+    a.q = tensor(d->q, d->q_ts, d->q_hs, es); a.k = tensor(d->k, d->k_ts, d->k_hs, es); a.v = tensor(d->v, d->v_ts, d->v_hs, es);
+    a.dout = tensor(dout, do_ts, do_hs, es);
+    a.dq = tensor(dq, dq_ts, dq_hs, es); a.dk = tensor(dk, dk_ts, dk_hs, es); a.dv = tensor(dv, dv_ts, dv_hs, es);
+    a.lse = lse; a.delta = delta; a.maxima = maxima; a.part = (float*)(ws + p.part);
+    a.T = d->T; a.Hq = d->Hq; a.Hk = d->Hk; a.D = d->D; a.causal = d->causal; a.nmax = p.nmax; a.scale = d->scale;
+    const AttnTensor o = tensor(out, (int64_t)d->Hq * d->D, d->D, es);
+    const int pieces = d->D * es / 16;
+    if (d->prec == HSIDM_BF16) launch_delta<bf16>(a.dout, o, a.v, d, pieces, p.nmax, delta, maxima, s);
+    else if (d->prec == HSIDM_F16) launch_delta<f16>(a.dout, o, a.v, d, pieces, p.nmax, delta, maxima, s);
+    else launch_delta<float>(a.dout, o, a.v, d, pieces, p.nmax, delta, maxima, s);
+    a.splits = p.kv.splits;
+    a.tiles = (const AttnTile*)(p.kv.waves == 4 ? d->ktiles128 : d->ktiles64);
+    if (int rc = launch(d->prec, ATTN_BWD_KV, &a, p.kv, s)) return rc;
+    if (a.splits > 1) {
+        const int64_t one = d->T * d->Hk * d->D;
+        add_parts(d->prec, a.part, p.kv, 2 * one, d->T, d->Hk, d->D, a.dk, s);
+        add_parts(d->prec, a.part + one, p.kv, 2 * one, d->T, d->Hk, d->D, a.dv, s);
+    }
+    a.splits = p.q.splits;
+    a.tiles = (const AttnTile*)(p.q.waves == 4 ? d->qtiles128 : d->qtiles64);
+    if (int rc = launch(d->prec, ATTN_BWD_Q, &a, p.q, s)) return rc;
+    if (a.splits > 1) add_parts(d->prec, a.part, p.q, d->T * d->Hq * d->D, d->T, d->Hq, d->D, a.dq, s);
+    return (int)hipGetLastError();
+}

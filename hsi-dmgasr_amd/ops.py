@@ -7,6 +7,7 @@ device memory and the current stream.
 import ctypes as C
 import math
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -649,6 +650,90 @@ def qk_norm_rope(q, k, wq, wk, pos, axes, eps=1e-6):
         with _lib.on_device(q.device):
             _lib.check(_lib.lib().hsidm_qk_norm_rope(C.byref(d), oq.data_ptr(), ok.data_ptr(), _lib.stream_ptr()), "qk_norm_rope")
     return oq, ok
+
+
+class PackedSequences:
+    """How a batch's tokens fall into sequences: `lengths` tokens each, one sequence behind the other (none of them is possible too).
+    Holds the kernels' tile tables on the device; built once per set of lengths, ahead of any stream capture."""
+
+    def __init__(self, lengths, device="cuda"):
+        self.lengths = tuple(int(n) for n in lengths)
+        if any(n < 0 for n in self.lengths) or sum(self.lengths) > 0x7fffffff:
+            raise ValueError("hsidm: sequence lengths must not be negative, nor more than 2^31 - 1 tokens together")
+        self.total, self.longest = sum(self.lengths), max(self.lengths, default=0)
+        lens = np.asarray(self.lengths, dtype=np.int64)
+        first = np.cumsum(lens) - lens
+        parts, self._at = [], {}
+        for rows in (64, 128):
+            n = -(-lens // rows)
+            seq = np.repeat(np.arange(len(lens)), n)
+            row0 = (np.arange(len(seq)) - np.repeat(np.cumsum(n) - n, n)) * rows
+            table = np.stack([first[seq], lens[seq], row0, np.zeros_like(row0)], axis=1).astype(np.int32)
+            # most work first: without a mask every tile walks its whole sequence; causal query tiles walk the keys up to their own last
+            # row, causal key tiles the queries from their own first row on
+            work = {"full": lens[seq], "causal q": np.minimum(lens[seq], row0 + rows), "causal k": lens[seq] - row0}
+            for kind, w in work.items():
+                self._at[kind, rows] = sum(len(p) for p in parts)
+                parts.append(table[np.argsort(-w, kind="stable")])
+            setattr(self, "n%d" % rows, len(seq))
+        self._tables = torch.from_numpy(np.concatenate(parts)).to(device)
+        self.device = self._tables.device
+
+    def _tiles(self, kind, rows):
+        return self._tables.data_ptr() + 16 * self._at[kind, rows]
+
+
+def attn_desc(q, k, v, seqs, causal, scale):
+    """(descriptor, tensors it points into) of hsidm_attention_packed after checking every argument."""
+    if any(t.dim() != 3 for t in (q, k, v)) or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError("hsidm: q, k, v must be [T, heads, D] over the same tokens, got %s" % ([tuple(t.shape) for t in (q, k, v)],))
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError("hsidm: the query heads (%d) must be a multiple of the key heads (%d)" % (Hq, Hk))
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("hsidm: q, k, v must have one type, got %s, %s, %s" % (q.dtype, k.dtype, v.dtype))
+    tid = _lib.type_id(q.dtype)
+    if not 1 <= D <= 256 or D * q.element_size() % 16:
+        raise ValueError("hsidm: head size must be at most 256 with rows of whole 16 bytes, got %d elements of %s" % (D, q.dtype))
+    if T != seqs.total:
+        raise ValueError("hsidm: %d tokens, but the sequences have %d" % (T, seqs.total))
+    if any(t.device != q.device for t in (k, v)) or seqs.device != q.device:
+        raise ValueError("hsidm: q, k, v and the sequences must be on one device")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError("hsidm: scale must be positive, got %r" % (scale,))
+    base(q)
+    q, k, v = token_rows(q), token_rows(k), token_rows(v)
+    d = _lib.AttnDesc()
+    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    (d.q_ts, d.q_hs), (d.k_ts, d.k_hs), (d.v_ts, d.v_hs) = _strides(q), _strides(k), _strides(v)
+    d.T, d.Hq, d.Hk, d.D, d.prec, d.causal, d.scale = T, Hq, Hk, D, tid, int(bool(causal)), scale
+    kinds = ("causal q", "causal k") if causal else ("full", "full")
+    d.qtiles64, d.qtiles128 = (seqs._tiles(kinds[0], r) for r in (64, 128))
+    d.ktiles64, d.ktiles128 = (seqs._tiles(kinds[1], r) for r in (64, 128))
+    d.n64, d.n128, d.longest = seqs.n64, seqs.n128, seqs.longest
+    return d, (q, k, v)
+
+
+def attention_packed(q, k, v, seqs, causal=False, scale=None, want_lse=False):
+    """softmax(scale * q k^T) v within every sequence of a packed batch: q [T, Hq, D], k / v [T, Hk, D] (Hk divides Hq; any strides, rows
+    on 16-byte boundaries are read in place), seqs a PackedSequences over the T tokens; causal: a token sees itself and what came
+    before; scale: 1/sqrt(D) unless given.  Any length - nothing of size length^2 is stored.  -> out [T, Hq, D] in q's type, with
+    want_lse also the log-sum-exp fp32 [Hq, T] that train_ops.attention_packed_bwd needs."""
+    d, keep = attn_desc(q, k, v, seqs, causal, scale)
+    T, Hq, D = q.shape
+    out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
+    if T:
+        L = _lib.lib()
+        with _lib.on_device(q.device):
+            nb = L.hsidm_attention_packed_workspace_bytes(C.byref(d))
+            if nb < 0:
+                _lib.check(int(nb), "attention_packed_workspace_bytes")
+            ws = torch.empty(int(nb), dtype=torch.uint8, device=q.device) if nb else None
+            _lib.check(L.hsidm_attention_packed(C.byref(d), out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), int(nb), _lib.stream_ptr()), "attention_packed")
+    return (out, lse) if want_lse else out
 
 
 _offset_cache = {}

@@ -389,3 +389,36 @@ def qk_norm_rope_bwd(d_out_q, d_out_k, q, k, wq, wk, pos, axes, eps=1e-6, out=No
         _check(L.hsidm_qk_norm_rope_bwd(C.byref(d), ops.base(gq), ops.base(gk), ops.base(dq), dq.stride(0), dq.stride(1), ops.base(dk), dk.stride(0),
                                         dk.stride(1), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), int(nb), _lib.stream_ptr()), "qk_norm_rope_bwd")
     return dq, dk, dwq, dwk
+
+
+def attention_packed_bwd(do, q, k, v, out, lse, seqs, causal=False, scale=None, grads=None):
+    """Gradient of ops.attention_packed: (dq, dk, dv) in the inputs' type from the output's gradient do, the inputs, the output and its lse.
+    grads: optional (dq, dk, dv) to write into, [T, H, D] views with 16-byte aligned rows (slices of a dqkv)."""
+    d, keep = ops.attn_desc(q, k, v, seqs, causal, scale)
+    T, Hq, _ = q.shape
+    for t in (do, out):
+        if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("hsidm: do and out must be like q: %s %s, got %s %s" % (tuple(q.shape), q.dtype, tuple(t.shape), t.dtype))
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or lse.device != q.device:
+        raise ValueError("hsidm: lse must be attention_packed's fp32 [%d, %d], got %s %s" % (Hq, T, lse.dtype, tuple(lse.shape)))
+    if grads is None:
+        grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    for g, x in zip(grads, (q, k, v)):
+        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device or not ops.rows_aligned(g):
+            raise ValueError("hsidm: grads must be [T, H, D] tensors like q, k, v with 16-byte aligned rows")
+    dq, dk, dv = grads
+    if T == 0:
+        return dq, dk, dv
+    L = _lib.lib()
+    with _lib.on_device(q.device):
+        nb = L.hsidm_attention_packed_bwd_workspace_bytes(C.byref(d))
+        if nb < 0:
+            _check(int(nb), "attention_packed_bwd_workspace_bytes")
+        ws = torch.empty(int(nb), dtype=torch.uint8, device=q.device)
+        do, out, lse = ops.token_rows(do), ops._aligned(out), lse.contiguous()
+        args = []
+        for t in (do, dq, dk, dv):
+            args += [t.data_ptr(), *ops._strides(t)]
+        _check(L.hsidm_attention_packed_bwd(C.byref(d), out.data_ptr(), _lib.ptr(lse), *args, _lib.ptr(ws), int(nb), _lib.stream_ptr()),
+               "attention_packed_bwd")
+    return dq, dk, dv

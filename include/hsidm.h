@@ -219,6 +219,38 @@ int hsidm_film_affine(int prec, const void* x, const float* gamma_beta, void* ou
  */
 int hsidm_attention(int prec, const void* qkv, void* out, int B, int N, int C, void* stream);
 
+/* ---- attention over packed sequences ------------------------------------------------------------------------------------------
+ * T tokens of several sequences, one behind the other: q [T][Hq][D], k, v [T][Hk][D] (Hk divides Hq; query head h uses key head
+ * h / (Hq / Hk)); every token attends to the tokens of its own sequence - causal: to those up to itself.
+ *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j]) v[j],   lse[h][i] = log sum_j exp(scale * q[i][h] . k[j])   (fp32 [Hq][T], may be
+ *   NULL where no backward pass follows); scale > 0.
+ * D <= 256 with rows of whole 16 bytes (multiples of 8, fp32: of 4); the last axis of q, k, v is contiguous, token and head strides (in
+ * elements) are multiples of 16 bytes, bases 16-byte aligned; out [T][Hq][D] contiguous.  fp32 (exact fp32 products), bf16, fp16; scores,
+ * softmax and sums in fp32, probabilities rounded to the type ahead of their product with v.
+ * Tiles (device memory, built by the caller once per set of lengths): for tile heights 64 and 128, the row ranges of every sequence of one
+ * or more tokens - {first token of the sequence, its length, first row of the tile within it, 0} - n64 / n128 of them; qtiles: in the
+ * order query tiles should start (most work first), ktiles: key tiles.  longest: the longest sequence.  Rows that no tile covers are not
+ * written.
+ * Values of k and v must be finite where a LATER token of the same 128-row tile is masked out for an earlier one (0 * inf is NaN).
+ * Backward: from out, lse and dout, recomputing the scores: dq, dk, dv (strided like their tensors), dk / dv summed over the heads that
+ * share them; no atomics, fixed order.  Workspaces: the _workspace_bytes functions (forward: 0 unless the keys are split), 16-byte aligned. */
+typedef struct hsidm_attn_tile { int32_t start, len, row0, reserved; } hsidm_attn_tile;
+typedef struct hsidm_attn_desc {
+    const void *q, *k, *v;
+    int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+    int64_t T;
+    const hsidm_attn_tile *qtiles64, *qtiles128, *ktiles64, *ktiles128;
+    int32_t n64, n128, longest;
+    int32_t Hq, Hk, D, prec, causal;
+    float scale;
+} hsidm_attn_desc;
+int64_t hsidm_attention_packed_workspace_bytes(const hsidm_attn_desc* d);
+int hsidm_attention_packed(const hsidm_attn_desc* d, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t hsidm_attention_packed_bwd_workspace_bytes(const hsidm_attn_desc* d);
+int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* out, const float* lse, const void* dout, int64_t do_ts, int64_t do_hs,
+                               void* dq, int64_t dq_ts, int64_t dq_hs, void* dk, int64_t dk_ts, int64_t dk_hs, void* dv, int64_t dv_ts,
+                               int64_t dv_hs, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- RMS norm of queries and keys per head + rotation by positions with several axes, one pass -------------------------------
  * For every token t < T and head of q ([T][Hq][D]) and k ([T][Hk][D]):
  *   n = x * rsqrt(mean(x^2) + eps) * w (w fp32 [D], one for q and one for k), then pair (n[p], n[p + D/2]), p < P = sum of sections, is
