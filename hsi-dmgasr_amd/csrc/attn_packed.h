@@ -182,6 +182,22 @@ __device__ __forceinline__ void store_column(T* out, const f32x16& acc, float f,
     }
 }
 
+// what rounding acc * f to the type left behind, rounded to the type itself
+template <typename T>
+__device__ __forceinline__ void store_residual(T* out, const f32x16& acc, float f, int d0, int h, int D) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int d = d0 + 8 * g + 4 * h;
+        if (d < D) {
+            typedef T vec __attribute__((ext_vector_type(4)));
+            vec v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { const float x = acc[4 * g + i] * f; v[i] = (T)(x - (float)(T)x); }
+            *reinterpret_cast<vec*>(out + d) = v;
+        }
+    }
+}
+
 // Workgroup -> (tile, head): all heads of a tile follow each other (the tiles come heaviest first, and a late heavy one would leave
 // the chip waiting), heads that share keys on one XCD (workgroups go to the eight XCDs in turn, each with an L2 of its own).
 __device__ __forceinline__ void which_tile(int heads, int& tile, int& head) {
@@ -194,6 +210,7 @@ __device__ __forceinline__ void which_tile(int heads, int& tile, int& head) {
 struct AttnFwdArgs {
     AttnTensor q, k, v;
     void* out;                       // [T][Hq][D] of the type, or fp32 [splits][T][Hq][D]
+    void* lo;                        // the rounding residual of out, like out; may be null (and is with splits: the join writes it)
     float* lse;                      // [Hq][T], or [splits][Hq][T]; may be null without splits
     const AttnTile* tiles;
     int64_t T;
@@ -209,6 +226,9 @@ template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_fwd_kernel(AttnFwdArgs a) {
     typedef Row<T, DP> R;
     constexpr int BN = R::BYTES <= 256 ? 64 : 32, ND = DP / 32, TILE = BN * R::BYTES;
+    // Where the accumulators spill over into the second half of the register file, a jump around work on them costs a move of every one of
+    // them on either way: such kernels do masked tiles too and rescale every time.
+    constexpr bool SKIP = R::BYTES <= 256;
     extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, h = lane >> 5;
     int ti, head;
@@ -240,7 +260,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
     for (int t = t0; t < t1; ++t) {
         const int buf = (t - t0) & 1, k0 = t * BN;
         if (t + 1 < t1) stage(t + 1, buf ^ 1);
-        if (q0 < len && (!a.causal || k0 <= q0 + 31)) {              // (uniform over the wave)
+        if (!SKIP || (q0 < len && (!a.causal || k0 <= q0 + 31))) {   // (uniform over the wave)
             const char* kt = lds + buf * 2 * TILE;
             const char* vt = kt + TILE;
             f32x16 s[BN / 32];
@@ -260,7 +280,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
 #pragma unroll
                 for (int j = 0; j < 16; ++j) mt = fmaxf(mt, s[b][j]);
             mt = both_halves_max(mt);
-            if (__any(!((mt - m) * c <= 8.0f) && mt != -INFINITY)) {
+            if (!SKIP || __any(!((mt - m) * c <= 8.0f) && mt != -INFINITY)) {
                 const float mn = fmaxf(m, mt), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
                 m = mn;
                 l *= f;
@@ -297,6 +317,11 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
         T* out = reinterpret_cast<T*>(a.out) + (token * a.Hq + head) * a.D;
 #pragma unroll
         for (int d = 0; d < ND; ++d) store_column<T>(out, o[d], inv, 32 * d, h, a.D);
+        if (sizeof(T) == 2 && a.lo) {
+            T* lo = reinterpret_cast<T*>(a.lo) + (token * a.Hq + head) * a.D;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) store_residual<T>(lo, o[d], inv, 32 * d, h, a.D);
+        }
     }
     if (a.lse && h == 0) a.lse[((int64_t)blockIdx.y * a.Hq + head) * a.T + token] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
 }
@@ -358,6 +383,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 128 ? 2 : 1)) void a
     which_tile(a.Hk, ti, kvh);
     const AttnTile tile = a.tiles[ti];
     const int len = tile.len, k0 = tile.row0 + wave * 32, group = a.Hq / a.Hk, pieces = a.D * (int)sizeof(T) / 16;
+    // this workgroup's work: the query tiles that see its keys, for every head of the group, one head behind the other
     const int tq0 = a.causal ? tile.row0 / BQ : 0, ntq = (len + BQ - 1) / BQ - tq0, work = ntq * group;
     const int per = (work + a.splits - 1) / a.splits, w0 = blockIdx.y * per, w1 = min(work, w0 + per);
     const int key = k0 + lr, keyc = min(key, len - 1);
@@ -392,36 +418,44 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 128 ? 2 : 1)) void a
         const char* qt = lds + buf * BUF;
         const char* gt = qt + TILE;
         const float* rows = reinterpret_cast<const float*>(qt + 2 * TILE);
-        if (k0 < len) {
+        // (no wave skips a tile: a jump around the products would have the accumulators change registers on either way)
 #pragma unroll
-            for (int b = 0; b < BQ / 32; ++b) {
-                if (q0 + 32 * b >= len || (a.causal && q0 + 32 * b + 31 < k0)) continue;       // (uniform over the wave)
-                f32x16 s, dp;
-                zero16(s); zero16(dp);
-                row_product<T, DP>(s, qt, 32 * b, at, kf);
-                row_product<T, DP>(dp, gt, 32 * b, at, vf);
-                const bool edge = q0 + 32 * b + 32 > len || (a.causal && q0 + 32 * b < k0 + 31);
+        for (int b = 0; b < BQ / 32; ++b) {
+            const char *qb = qt + b * 32 * R::BYTES, *gb = gt + b * 32 * R::BYTES;
+            const float* rb = rows + 32 * b + 4 * h;
+            f32x16 s, dp;
+            zero16(s); zero16(dp);
+            row_product<T, DP>(s, qb, 0, at, kf);
+            row_product<T, DP>(dp, gb, 0, at, vf);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(rows + 32 * b + 8 * g + 4 * h);
-                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(rows + 64 + 32 * b + 8 * g + 4 * h);
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(rb + 8 * g);
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(rb + 64 + 8 * g);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = 4 * g + i, q = q0 + 32 * b + 8 * g + 4 * h + i;
-                        float p = __builtin_amdgcn_exp2f(fmaf(s[j], c, GradScale<T>::p_shift - l4[i] * kLog2e));
-                        float x = p * (dp[j] - d4[i]);
-                        if constexpr (GradScale<T>::on) x *= f;
-                        if (edge && (q >= len || (a.causal && q < key))) { p = 0.f; x = 0.f; }
-                        s[j] = p; dp[j] = x;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const int j = 4 * g + i;
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[j], c, GradScale<T>::p_shift - l4[i] * kLog2e));
+                    float x = p * (dp[j] - d4[i]);
+                    if constexpr (GradScale<T>::on) x *= f;
+                    s[j] = p; dp[j] = x;
                 }
-                ColFrag<T> pf, sf;
-                pf.set(s); sf.set(dp);
+            }
+            const int qr = q0 + 32 * b;
+            if (qr + 32 > len || (a.causal && qr < k0 + 31)) {       // (a pass of its own: selects, no branch per element)
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    col_product<T, DP>(dv[d], gt + dbytes, 32 * b, d, at, pf);
-                    col_product<T, DP>(dk[d], qt + dbytes, 32 * b, d, at, sf);
+                for (int j = 0; j < 16; ++j) {
+                    const int q = qr + 8 * (j >> 2) + 4 * h + (j & 3);
+                    const bool gone = q >= len || (a.causal && q < key);
+                    s[j] = gone ? 0.f : s[j];
+                    dp[j] = gone ? 0.f : dp[j];
                 }
+            }
+            ColFrag<T> pf, sf;
+            pf.set(s); sf.set(dp);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                col_product<T, DP>(dv[d], gb + dbytes, 0, d, at, pf);
+                col_product<T, DP>(dk[d], qb + dbytes, 0, d, at, sf);
             }
         }
         wait_loads();
@@ -453,6 +487,7 @@ template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_bwd_q_kernel(AttnBwdArgs a) {
     typedef Row<T, DP> R;
     constexpr int BN = R::BYTES <= 256 ? 64 : 32, ND = DP / 32, TILE = BN * R::BYTES;
+    constexpr bool SKIP = R::BYTES <= 256;                           // (as in the forward kernel)
     extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, h = lane >> 5;
     int ti, head;
@@ -489,11 +524,11 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
         if (t + 1 < t1) stage(t + 1, buf ^ 1);
         const char* kt = lds + buf * 2 * TILE;
         const char* vt = kt + TILE;
-        if (q0 < len) {
+        if (!SKIP || q0 < len) {
             const int last = a.causal ? min(len - 1, row) : len - 1;
 #pragma unroll
             for (int b = 0; b < BN / 32; ++b) {
-                if (k0 + 32 * b >= len || (a.causal && k0 + 32 * b > q0 + 31)) continue;       // (uniform over the wave)
+                if (SKIP && (k0 + 32 * b >= len || (a.causal && k0 + 32 * b > q0 + 31))) continue;       // (uniform over the wave)
                 f32x16 s, dp;
                 zero16(s); zero16(dp);
                 row_product<T, DP>(s, kt, 32 * b, at, qf);
@@ -503,8 +538,11 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
                 for (int j = 0; j < 16; ++j) {
                     float x = __builtin_amdgcn_exp2f(fmaf(s[j], c, -lse2)) * (dp[j] - delta);
                     if constexpr (GradScale<T>::on) x *= f;
-                    if (edge && k0 + 32 * b + 8 * (j >> 2) + 4 * h + (j & 3) > last) x = 0.f;
                     s[j] = x;
+                }
+                if (edge) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[j] = k0 + 32 * b + 8 * (j >> 2) + 4 * h + (j & 3) > last ? 0.f : s[j];
                 }
                 ColFrag<T> sf;
                 sf.set(s);

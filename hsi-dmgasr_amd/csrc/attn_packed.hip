@@ -1,6 +1,7 @@
 // Attention over packed sequences: the C entry points, the choice of tile and split, and the small kernels around the main ones
 // (attn_packed.h): joining split key ranges, the backward pass's row sums, adding split partial gradients.
 #include "attn_packed.h"
+#include <cmath>
 
 namespace hsidm {
 
@@ -8,7 +9,7 @@ namespace hsidm {
 // exp(lse_s - lse).  Four elements a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, const float* __restrict__ plse, int S, int64_t T_, int Hq, int D,
-                                                        T* __restrict__ out, float* __restrict__ lse) {
+                                                        T* __restrict__ out, T* __restrict__ lo, float* __restrict__ lse) {
     const int per_row = D / 4;
     const int64_t n = T_ * Hq * per_row, rows = T_ * Hq;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
@@ -28,11 +29,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
             for (int k = 0; k < 4; ++k) v[k] += w * x[k];
         }
         typedef T vec __attribute__((ext_vector_type(4)));
-        vec r;
+        vec r, e;
         const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) r[k] = (T)(v[k] * inv);
+        for (int k = 0; k < 4; ++k) { v[k] *= inv; r[k] = (T)v[k]; e[k] = (T)(v[k] - (float)r[k]); }
         *reinterpret_cast<vec*>(out + row * D + d) = r;
+        if (lo) *reinterpret_cast<vec*>(lo + row * D + d) = e;
         if (lse && d == 0) lse[at] = mm + logf(l);
     }
 }
@@ -59,12 +61,13 @@ __global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__
     }
 }
 
-// delta[h][t] = sum_d dO O per row; fp16: also this workgroup's largest |dO|^2 and |V|^2 (GradScale).  `group` lanes, a power of two that
+// delta[h][t] = sum_d dO O per row, O with its rounding residual where the forward pass kept it (without it, delta's error is as large as
+// that of rounding dS and adds to it in dQ and dK: 1.55 ... 1.7 instead of 1.4 times the output's own rounding); fp16: also this workgroup's largest |dO|^2 and |V|^2 (GradScale).  `group` lanes, a power of two that
 // covers a row's 16-byte pieces, share a row.
 constexpr int kDeltaBlocks = 512;
 
 template <typename T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTensor o, AttnTensor v, int64_t T_, int Hq, int Hk, int pieces, int group,
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTensor o, const char* __restrict__ lo, AttnTensor v, int64_t T_, int Hq, int Hk, int pieces, int group,
                                                          float* __restrict__ delta, float* __restrict__ maxima) {
     constexpr int E = 16 / (int)sizeof(T);
     typedef T vec __attribute__((ext_vector_type(E)));
@@ -84,6 +87,11 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTe
             const vec y = *reinterpret_cast<const vec*>(o.p + token * o.ts + head * o.hs + sub * 16);
 #pragma unroll
             for (int k = 0; k < E; ++k) { dot += (float)x[k] * (float)y[k]; sq += (float)x[k] * (float)x[k]; }
+            if (sizeof(T) == 2 && lo) {
+                const vec z = *reinterpret_cast<const vec*>(lo + token * o.ts + head * o.hs + sub * 16);
+#pragma unroll
+                for (int k = 0; k < E; ++k) dot += (float)x[k] * (float)z[k];
+            }
         }
         dot = sum(dot);
         if (GradScale<T>::on) ma = fmaxf(ma, sum(sq));
@@ -113,21 +121,47 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTe
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 struct Cut { int waves, ntiles, splits; };
+static int row_bytes(int D, int es) { return (D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256) * es; }
+static int tile_rows(int D, int es) { return row_bytes(D, es) <= 256 ? 64 : 32; }
 
-// Tile height and split of the long axis.  128-row tiles (4 waves) where they give every CU a workgroup, else 64-row ones.  The walked axis
-// (`steps` tiles of the longest sequence) is split, into shares of at least four tiles, while the waves do not reach two per SIMD.
-static Cut cut_work(int heads, int n64, int n128, int64_t steps) {
+// Tile height and split of the walked axis.  128-row tiles (4 waves) where they fill half the chip or the walk is long enough to split,
+// else 64-row ones.  The walk is split where that pays by a coarse estimate of the time, in seconds, per number of shares:
+//   tiles of equal work: rounds of resident workgroups times a share's steps;
+//   unequal ones (causal, ragged; heaviest first): all work at the full rate, and 0.45 of the longest share at the end, alone;
+//   plus the shares' partial sums, written in fp32 and read again.
+// The rates are what the kernels reach (a step of the measured cases comes out within 15 %); shares stay at four steps or more.
+struct Walk { int resident, products; bool kv; };            // workgroups of four waves per CU (by registers), matrix products per tile pair
+static Cut cut_work(const hsidm_attn_desc* d, int es, const Walk& k) {
+    const int heads = k.kv ? d->Hk : d->Hq, walks = k.kv ? d->Hq / d->Hk : 1, rows = tile_rows(d->D, es), width = row_bytes(d->D, es) / es;
+    const int64_t steps = (d->longest + rows - 1) / rows * walks;
+    const double cus = device_cus(), rate = es == 4 ? 105e12 : width <= 32 ? 250e12 : width <= 64 ? 600e12 : 750e12;
     Cut c;
-    c.waves = (int64_t)n128 * heads >= device_cus() ? 4 : 2;
-    c.ntiles = c.waves == 4 ? n128 : n64;
-    const int64_t waves = (int64_t)c.ntiles * heads * c.waves, want = (int64_t)device_cus() * 8;
-    int64_t s = waves > 0 ? want / waves : 1;
-    if (s > steps / 4) s = steps / 4;
-    if (s > 16) s = 16;
-    c.splits = s > 1 ? (int)s : 1;
+    c.waves = (double)d->n128 * heads >= 0.5 * cus || steps >= 16 ? 4 : 2;
+    c.ntiles = c.waves == 4 ? d->n128 : d->n64;
+    const int tile = 32 * c.waves;
+    const double slots = cus * k.resident * (4 / c.waves), n = (double)c.ntiles * heads;
+    const double step = 2.0 * rows * tile * width * k.products;                            // flops
+    const double total = d->pairs * heads * walks / ((double)tile * rows) * step;
+    const double bytes = 2.0 * 4.0 * d->T * heads * d->D * (k.kv ? 2 : 1);                 // of one share's sums, there and back
+    const bool equal = total > 0.9 * n * steps * step;
+    double best = 1e300;
+    c.splits = 1;
+    for (int s = 1; s <= 16 && (s == 1 || steps / s >= 4); ++s) {
+        const double share = (double)((steps + s - 1) / s) * step;
+        double t = equal ? std::ceil(n * s / slots) * share * slots / rate : total / rate + 0.45 * share * cus / rate;
+        if (s > 1) t += s * bytes / 4.5e12 + 5e-6;
+        if (t < 0.97 * best) { best = t; c.splits = s; }
+    }
     return c;
 }
-static int tile_rows(int D, int es) { return (D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256) * es <= 256 ? 64 : 32; }
+static Cut cut_queries(const hsidm_attn_desc* d, int es, int products) {
+    const int rb = row_bytes(d->D, es);
+    return cut_work(d, es, {rb <= 128 ? 3 : rb <= 256 ? 2 : 1, products, false});
+}
+static Cut cut_keys(const hsidm_attn_desc* d, int es) {
+    const int rb = row_bytes(d->D, es);
+    return cut_work(d, es, {rb <= 128 ? 2 : 1, d->D > 128 ? 6 : 4, true});
+}
 
 static bool rows_ok(const void* p, int64_t ts, int64_t hs, int es) {
     return p && (uintptr_t)p % 16 == 0 && ts >= 0 && hs >= 0 && ts * es % 16 == 0 && hs * es % 16 == 0;
@@ -139,7 +173,7 @@ static int check_attn(const hsidm_attn_desc* d, int& es) {
     if (d->D < 16 / es || d->D > 256 || d->D * es % 16) return HSIDM_E_BADARG;
     if (!(d->scale > 0.f) || !(d->scale < 1e30f)) return HSIDM_E_BADARG;
     if (!rows_ok(d->q, d->q_ts, d->q_hs, es) || !rows_ok(d->k, d->k_ts, d->k_hs, es) || !rows_ok(d->v, d->v_ts, d->v_hs, es)) return HSIDM_E_BADARG;
-    if (!d->qtiles64 || !d->qtiles128 || !d->ktiles64 || !d->ktiles128 || d->n64 <= 0 || d->n128 <= 0 || d->longest <= 0) return HSIDM_E_BADARG;
+    if (!d->qtiles64 || !d->qtiles128 || !d->ktiles64 || !d->ktiles128 || d->n64 <= 0 || d->n128 <= 0 || d->longest <= 0 || !(d->pairs > 0)) return HSIDM_E_BADARG;
     if ((int64_t)d->n64 * d->Hq > 0x7fffffff) return HSIDM_E_UNSUPPORTED;
     return 0;
 }
@@ -155,9 +189,8 @@ static unsigned blocks_for(int64_t n) { const int64_t b = (n + 255) / 256; retur
 struct BwdPlan { Cut q, kv; int64_t delta, maxima, part, bytes; int nmax; };
 static BwdPlan bwd_plan(const hsidm_attn_desc* d, int es) {
     BwdPlan p;
-    const int64_t steps = (d->longest + tile_rows(d->D, es) - 1) / tile_rows(d->D, es);
-    p.q = cut_work(d->Hq, d->n64, d->n128, steps);
-    p.kv = cut_work(d->Hk, d->n64, d->n128, steps * (d->Hq / d->Hk));
+    p.q = cut_queries(d, es, 3);
+    p.kv = cut_keys(d, es);
     int group = 1;
     while (group < d->D * es / 16) group *= 2;
     const int64_t rows = d->T * d->Hq, blocks = (rows * group + 255) / 256;
@@ -172,11 +205,11 @@ static BwdPlan bwd_plan(const hsidm_attn_desc* d, int es) {
 }
 
 template <typename T>
-static void launch_delta(const AttnTensor& dout, const AttnTensor& o, const AttnTensor& v, const hsidm_attn_desc* d, int pieces, int nmax, float* delta,
+static void launch_delta(const AttnTensor& dout, const AttnTensor& o, const void* lo, const AttnTensor& v, const hsidm_attn_desc* d, int pieces, int nmax, float* delta,
                          float* maxima, hipStream_t s) {
     int group = 1;
     while (group < pieces) group *= 2;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_delta_kernel<T>), dim3(nmax), dim3(256), 0, s, dout, o, v, d->T, d->Hq, d->Hk, pieces, group, delta, maxima);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_delta_kernel<T>), dim3(nmax), dim3(256), 0, s, dout, o, (const char*)lo, v, d->T, d->Hq, d->Hk, pieces, group, delta, maxima);
 }
 template <typename T>
 static void launch_add(const float* part, const Cut& c, int64_t share, int64_t T_, int H, int D, const AttnTensor& out, hipStream_t s) {
@@ -195,21 +228,22 @@ using namespace hsidm;
 extern "C" int64_t hsidm_attention_packed_workspace_bytes(const hsidm_attn_desc* d) {
     int es;
     if (int rc = check_attn(d, es)) return rc;
-    const Cut c = cut_work(d->Hq, d->n64, d->n128, (d->longest + tile_rows(d->D, es) - 1) / tile_rows(d->D, es));
+    const Cut c = cut_queries(d, es, 2);
     return c.splits > 1 ? (int64_t)c.splits * d->T * d->Hq * (d->D + 1) * 4 : 0;
 }
 
-extern "C" int hsidm_attention_packed(const hsidm_attn_desc* d, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int hsidm_attention_packed(const hsidm_attn_desc* d, void* out, void* out_lo, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
     int es;
     if (int rc = check_attn(d, es)) return rc;
-    if (!rows_ok(out, 0, 0, es)) return HSIDM_E_BADARG;
-    const Cut c = cut_work(d->Hq, d->n64, d->n128, (d->longest + tile_rows(d->D, es) - 1) / tile_rows(d->D, es));
+    if (!rows_ok(out, 0, 0, es) || (uintptr_t)out_lo % 16) return HSIDM_E_BADARG;
+    const Cut c = cut_queries(d, es, 2);
     const int64_t rows = d->T * d->Hq;
     if (c.splits > 1 && (!rows_ok(workspace, 0, 0, 4) || workspace_bytes < c.splits * rows * (d->D + 1) * 4)) return HSIDM_E_BADARG;
     AttnFwdArgs a;
     a.q = tensor(d->q, d->q_ts, d->q_hs, es); a.k = tensor(d->k, d->k_ts, d->k_hs, es); a.v = tensor(d->v, d->v_ts, d->v_hs, es);
     float* part = (float*)workspace;
     a.out = c.splits > 1 ? (void*)part : out;
+    a.lo = c.splits > 1 ? nullptr : out_lo;
     a.lse = c.splits > 1 ? part + c.splits * rows * d->D : lse;
     a.tiles = (const AttnTile*)(c.waves == 4 ? d->qtiles128 : d->qtiles64);
     a.T = d->T; a.Hq = d->Hq; a.Hk = d->Hk; a.D = d->D; a.causal = d->causal; a.splits = c.splits; a.scale = d->scale;
@@ -218,7 +252,7 @@ extern "C" int hsidm_attention_packed(const hsidm_attn_desc* d, void* out, float
     if (c.splits > 1) {
         const dim3 grid(blocks_for(rows * d->D / 4));
         const float* pl = part + c.splits * rows * d->D;
-#define JOIN(OUT) hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_join_kernel<OUT>), grid, dim3(256), 0, s, (const float*)part, pl, c.splits, d->T, d->Hq, d->D, (OUT*)out, lse)
+#define JOIN(OUT) hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_join_kernel<OUT>), grid, dim3(256), 0, s, (const float*)part, pl, c.splits, d->T, d->Hq, d->D, (OUT*)out, (OUT*)out_lo, lse)
         if (d->prec == HSIDM_BF16) JOIN(bf16);
         else if (d->prec == HSIDM_F16) JOIN(f16);
         else JOIN(float);
@@ -233,12 +267,12 @@ extern "C" int64_t hsidm_attention_packed_bwd_workspace_bytes(const hsidm_attn_d
     return bwd_plan(d, es).bytes;
 }
 
-extern "C" int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* out, const float* lse, const void* dout, int64_t do_ts, int64_t do_hs,
+extern "C" int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* out, const void* out_lo, const float* lse, const void* dout, int64_t do_ts, int64_t do_hs,
                                           void* dq, int64_t dq_ts, int64_t dq_hs, void* dk, int64_t dk_ts, int64_t dk_hs, void* dv, int64_t dv_ts,
                                           int64_t dv_hs, void* workspace, int64_t workspace_bytes, void* stream) {
     int es;
     if (int rc = check_attn(d, es)) return rc;
-    if (!lse || !rows_ok(out, 0, 0, es) || !rows_ok(dout, do_ts, do_hs, es) || !rows_ok(dq, dq_ts, dq_hs, es) || !rows_ok(dk, dk_ts, dk_hs, es) ||
+    if (!lse || !rows_ok(out, 0, 0, es) || (uintptr_t)out_lo % 16 || !rows_ok(dout, do_ts, do_hs, es) || !rows_ok(dq, dq_ts, dq_hs, es) || !rows_ok(dk, dk_ts, dk_hs, es) ||
         !rows_ok(dv, dv_ts, dv_hs, es))
         return HSIDM_E_BADARG;
     const BwdPlan p = bwd_plan(d, es);
@@ -254,9 +288,9 @@ extern "C" int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* 
     a.T = d->T; a.Hq = d->Hq; a.Hk = d->Hk; a.D = d->D; a.causal = d->causal; a.nmax = p.nmax; a.scale = d->scale;
     const AttnTensor o = tensor(out, (int64_t)d->Hq * d->D, d->D, es);
     const int pieces = d->D * es / 16;
-    if (d->prec == HSIDM_BF16) launch_delta<bf16>(a.dout, o, a.v, d, pieces, p.nmax, delta, maxima, s);
-    else if (d->prec == HSIDM_F16) launch_delta<f16>(a.dout, o, a.v, d, pieces, p.nmax, delta, maxima, s);
-    else launch_delta<float>(a.dout, o, a.v, d, pieces, p.nmax, delta, maxima, s);
+    if (d->prec == HSIDM_BF16) launch_delta<bf16>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
+    else if (d->prec == HSIDM_F16) launch_delta<f16>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
+    else launch_delta<float>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
     a.splits = p.kv.splits;
     a.tiles = (const AttnTile*)(p.kv.waves == 4 ? d->ktiles128 : d->ktiles64);
     if (int rc = launch(d->prec, ATTN_BWD_KV, &a, p.kv, s)) return rc;

@@ -4,6 +4,7 @@ Tensors here are the path's internal representation: NHWC activations (torch sha
 the storage type of the precision mode (bf16 / fp32), fp32 everywhere else.  torch only supplies
 device memory and the current stream.
 """
+import collections
 import ctypes as C
 import math
 
@@ -571,10 +572,15 @@ def base(t):
     return t.data_ptr()
 
 
-def rows_aligned(t):
-    """Does every (token, head) row of [T, H, D] start on a 16-byte boundary, contiguous along D?"""
+def rows_strided(t):
+    """Are the (token, head) rows of [T, H, D] contiguous along D and whole multiples of 16 bytes apart?"""
     es = t.element_size()
-    return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] <= 1 or (t.stride(i) * es) % 16 == 0 and t.stride(i) > 0 for i in (0, 1))
+    return (t.stride(2) == 1 or t.shape[2] == 1) and all(t.shape[i] <= 1 or (t.stride(i) * es) % 16 == 0 and t.stride(i) > 0 for i in (0, 1))
+
+
+def rows_aligned(t):
+    """rows_strided, on 16-byte boundaries."""
+    return t.data_ptr() % 16 == 0 and rows_strided(t)
 
 
 def token_rows(t):
@@ -603,10 +609,11 @@ class RotaryAxes:
             raise ValueError("hsidm: base must be greater than one, got %r" % (base,))
         turns = [float(base) ** (-j / n) / (2.0 * math.pi) for n in self.sections for j in range(n)]
         self.freq = torch.tensor(turns or [0.0], dtype=torch.float64).to(device)
+        self._plans = {}                                  # (rope_desc)
 
 
-def rope_desc(q, k, wq, wk, pos, axes, eps):
-    """(descriptor, tensors it points into) of hsidm_qk_norm_rope after checking every argument."""
+def _check_rope(q, k, wq, wk, pos, axes, eps):
+    """Everything about a call but its addresses: (descriptor without them, backward workspace bytes, whether all tensors are read in place)."""
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[1] < 1 or k.shape[1] < 1:
         raise ValueError("hsidm: q and k must be [T, heads, D] over the same tokens, got %s and %s" % (tuple(q.shape), tuple(k.shape)))
     T, Hq, D = q.shape
@@ -625,14 +632,43 @@ def rope_desc(q, k, wq, wk, pos, axes, eps):
     if not float(eps) >= 0:
         raise ValueError("hsidm: eps must not be negative, got %r" % (eps,))
     base(q)
-    q, k, wq, wk, pos = token_rows(q), token_rows(k), _aligned(wq), _aligned(wk), pos.contiguous()
     d = _lib.RopeDesc()
-    d.q, d.k, d.wq, d.wk, d.pos, d.freq = (t.data_ptr() for t in (q, k, wq, wk, pos, axes.freq))
-    (d.q_ts, d.q_hs), (d.k_ts, d.k_hs) = _strides(q), _strides(k)
     d.T, d.Hq, d.Hk, d.D, d.axes, d.prec, d.eps = T, Hq, k.shape[1], D, len(axes.sections), tid, float(eps)
+    d.freq = axes.freq.data_ptr()
     for i, n in enumerate(axes.sections):
         d.sections[i] = n
-    return d, (q, k, wq, wk, pos)
+    nb = 0
+    if T:
+        d.q = d.k = d.wq = d.wk = d.pos = d.freq & ~15        # (any aligned address: the size does not depend on it)
+        nb = _lib.lib().hsidm_qk_norm_rope_bwd_workspace_bytes(C.byref(d))
+        if nb < 0:
+            _lib.check(int(nb), "qk_norm_rope_bwd_workspace_bytes")
+    in_place = rows_strided(q) and rows_strided(k) and all(t.is_contiguous() for t in (wq, wk, pos))
+    if in_place:
+        (d.q_ts, d.q_hs), (d.k_ts, d.k_hs) = _strides(q), _strides(k)
+    return d, nb, in_place
+
+
+def rope_desc(q, k, wq, wk, pos, axes, eps):
+    """(descriptor, backward workspace bytes, tensors it points into) of hsidm_qk_norm_rope.  The checks of a combination of shapes,
+    strides, types and devices are made once per RotaryAxes; the addresses are each call's own."""
+    key = (q.shape, k.shape, wq.shape, wk.shape, pos.shape, q.stride(), k.stride(), wq.stride(), wk.stride(), pos.stride(), q.dtype, k.dtype, wq.dtype,
+           wk.dtype, pos.dtype, q.device, k.device, wq.device, wk.device, pos.device, eps)
+    plan = axes._plans.get(key)
+    if plan is None:
+        plan = _check_rope(q, k, wq, wk, pos, axes, eps)
+        if len(axes._plans) >= 64:
+            axes._plans.clear()
+        axes._plans[key] = plan
+    d = _lib.RopeDesc.from_buffer_copy(plan[0])
+    ptrs = [t.data_ptr() for t in (q, k, wq, wk)]
+    if not plan[2] or (ptrs[0] | ptrs[1] | ptrs[2] | ptrs[3]) & 15:
+        q, k, wq, wk, pos = token_rows(q), token_rows(k), _aligned(wq), _aligned(wk), pos.contiguous()
+        ptrs = [t.data_ptr() for t in (q, k, wq, wk)]
+        (d.q_ts, d.q_hs), (d.k_ts, d.k_hs) = _strides(q), _strides(k)
+    d.q, d.k, d.wq, d.wk = ptrs
+    d.pos = pos.data_ptr()
+    return d, plan[1], (q, k, wq, wk, pos)
 
 
 def _aligned(t):
@@ -644,9 +680,9 @@ def qk_norm_rope(q, k, wq, wk, pos, axes, eps=1e-6):
     """RMS norm of every query and key head (weights wq, wk fp32 [D]) and its rotation by the token's positions, one launch:
     q [T, Hq, D], k [T, Hk, D] (any strides; rows on 16-byte boundaries are read in place), pos int32 [T, axes], axes a RotaryAxes.
     -> two contiguous tensors of q's type.  Gradient: train_ops.qk_norm_rope_bwd."""
-    d, keep = rope_desc(q, k, wq, wk, pos, axes, eps)
-    oq, ok = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if q.shape[0]:
+    d, _, keep = rope_desc(q, k, wq, wk, pos, axes, eps)
+    oq, ok = q.new_empty(q.shape), k.new_empty(k.shape)
+    if d.T:
         with _lib.on_device(q.device):
             _lib.check(_lib.lib().hsidm_qk_norm_rope(C.byref(d), oq.data_ptr(), ok.data_ptr(), _lib.stream_ptr()), "qk_norm_rope")
     return oq, ok
@@ -678,13 +714,19 @@ class PackedSequences:
             setattr(self, "n%d" % rows, len(seq))
         self._tables = torch.from_numpy(np.concatenate(parts)).to(device)
         self.device = self._tables.device
+        self._plans = {}                                  # (attn_desc)
+
+    def pairs(self, causal):
+        """(query, key) pairs of one head."""
+        return sum(n * (n + 1) // 2 if causal else n * n for n in self.lengths)
 
     def _tiles(self, kind, rows):
         return self._tables.data_ptr() + 16 * self._at[kind, rows]
 
 
-def attn_desc(q, k, v, seqs, causal, scale):
-    """(descriptor, tensors it points into) of hsidm_attention_packed after checking every argument."""
+def _check_attn(q, k, v, seqs, causal, scale):
+    """Everything about an attention call but its addresses: (descriptor without them, forward / backward workspace bytes, whether q, k, v
+    are read in place)."""
     if any(t.dim() != 3 for t in (q, k, v)) or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError("hsidm: q, k, v must be [T, heads, D] over the same tokens, got %s" % ([tuple(t.shape) for t in (q, k, v)],))
     T, Hq, D = q.shape
@@ -704,36 +746,65 @@ def attn_desc(q, k, v, seqs, causal, scale):
     if not 0.0 < scale < 1e30:
         raise ValueError("hsidm: scale must be positive, got %r" % (scale,))
     base(q)
-    q, k, v = token_rows(q), token_rows(k), token_rows(v)
     d = _lib.AttnDesc()
-    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    (d.q_ts, d.q_hs), (d.k_ts, d.k_hs), (d.v_ts, d.v_hs) = _strides(q), _strides(k), _strides(v)
     d.T, d.Hq, d.Hk, d.D, d.prec, d.causal, d.scale = T, Hq, Hk, D, tid, int(bool(causal)), scale
     kinds = ("causal q", "causal k") if causal else ("full", "full")
     d.qtiles64, d.qtiles128 = (seqs._tiles(kinds[0], r) for r in (64, 128))
     d.ktiles64, d.ktiles128 = (seqs._tiles(kinds[1], r) for r in (64, 128))
-    d.n64, d.n128, d.longest = seqs.n64, seqs.n128, seqs.longest
-    return d, (q, k, v)
+    d.n64, d.n128, d.longest, d.pairs = seqs.n64, seqs.n128, seqs.longest, seqs.pairs(causal)
+    in_place = rows_strided(q) and rows_strided(k) and rows_strided(v)
+    nb = (0, 0)
+    if T:
+        d.q = d.k = d.v = d.qtiles64 & ~15                # (any aligned address: the sizes do not depend on it)
+        nb = (_lib.lib().hsidm_attention_packed_workspace_bytes(C.byref(d)), _lib.lib().hsidm_attention_packed_bwd_workspace_bytes(C.byref(d)))
+        if min(nb) < 0:
+            _lib.check(int(min(nb)), "attention_packed_workspace_bytes")
+    if in_place:
+        (d.q_ts, d.q_hs), (d.k_ts, d.k_hs), (d.v_ts, d.v_hs) = _strides(q), _strides(k), _strides(v)
+    return d, nb[0], nb[1], in_place
+
+
+def attn_desc(q, k, v, seqs, causal, scale):
+    """(descriptor, forward workspace bytes, backward workspace bytes, tensors it points into) of hsidm_attention_packed.  The checks of
+    a combination of shapes, strides, types and devices are made once per PackedSequences; the addresses are each call's own."""
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device, v.device, causal, scale)
+    plan = seqs._plans.get(key)
+    if plan is None:
+        plan = _check_attn(q, k, v, seqs, causal, scale)
+        if len(seqs._plans) >= 64:
+            seqs._plans.clear()
+        seqs._plans[key] = plan
+    d = _lib.AttnDesc.from_buffer_copy(plan[0])
+    d.q, d.k, d.v = pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not plan[3] or (pq | pk | pv) & 15:
+        q, k, v = token_rows(q), token_rows(k), token_rows(v)
+        d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        (d.q_ts, d.q_hs), (d.k_ts, d.k_hs), (d.v_ts, d.v_hs) = _strides(q), _strides(k), _strides(v)
+    return d, plan[1], plan[2], (q, k, v)
+
+
+# what the backward pass needs beside the output: lse fp32 [Hq, T] = log sum_j exp(scale q.k), and (16-bit types) the output's rounding
+# residual, in its type and shape
+AttentionSaved = collections.namedtuple("AttentionSaved", "lse residual")
 
 
 def attention_packed(q, k, v, seqs, causal=False, scale=None, want_lse=False):
     """softmax(scale * q k^T) v within every sequence of a packed batch: q [T, Hq, D], k / v [T, Hk, D] (Hk divides Hq; any strides, rows
     on 16-byte boundaries are read in place), seqs a PackedSequences over the T tokens; causal: a token sees itself and what came
     before; scale: 1/sqrt(D) unless given.  Any length - nothing of size length^2 is stored.  -> out [T, Hq, D] in q's type, with
-    want_lse also the log-sum-exp fp32 [Hq, T] that train_ops.attention_packed_bwd needs."""
-    d, keep = attn_desc(q, k, v, seqs, causal, scale)
-    T, Hq, D = q.shape
-    out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
-    if T:
-        L = _lib.lib()
+    want_lse also the AttentionSaved that train_ops.attention_packed_bwd takes."""
+    d, nb, _, keep = attn_desc(q, k, v, seqs, causal, scale)
+    out = q.new_empty(q.shape)
+    lse = lo = None
+    if want_lse:
+        lse = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+        lo = q.new_empty(q.shape) if q.element_size() == 2 else None
+    if d.T:
         with _lib.on_device(q.device):
-            nb = L.hsidm_attention_packed_workspace_bytes(C.byref(d))
-            if nb < 0:
-                _lib.check(int(nb), "attention_packed_workspace_bytes")
-            ws = torch.empty(int(nb), dtype=torch.uint8, device=q.device) if nb else None
-            _lib.check(L.hsidm_attention_packed(C.byref(d), out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), int(nb), _lib.stream_ptr()), "attention_packed")
-    return (out, lse) if want_lse else out
+            ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
+            _lib.check(_lib.lib().hsidm_attention_packed(C.byref(d), out.data_ptr(), _lib.ptr(lo), _lib.ptr(lse), _lib.ptr(ws), nb, _lib.stream_ptr()),
+                       "attention_packed")
+    return (out, AttentionSaved(lse, lo)) if want_lse else out
 
 
 _offset_cache = {}

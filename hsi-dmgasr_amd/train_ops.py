@@ -293,10 +293,13 @@ def _is_dense(t):
     return True
 
 
+_data_ptr, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
+
+
 class TensorList:
     """The tensors of a gradient norm or clipping call, checked once: dense fp32 / bf16 / fp16 ROCm tensors of one device, mixed types
     as they come (None entries - parameters without a gradient - are left out).  A program that keeps its gradient tensors keeps the
-    list too; addresses and sizes are read again on every call, so tensors that were given new storage are followed."""
+    list too; addresses, sizes and types are read again on every call, so tensors that were given new storage are followed."""
 
     def __init__(self, tensors):
         tensors = [tensors] if torch.is_tensor(tensors) else [t for t in tensors if t is not None]
@@ -310,16 +313,19 @@ class TensorList:
         self.tensors = tensors
         self.device = tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
         self._key, self._items, self._disjoint = None, None, None
+        self.items()
 
     def items(self):
-        key = [(t.data_ptr(), t.shape, t.stride(), t.dtype) for t in self.tensors]
+        """The host array of hsidm_grad_norm, made again where a tensor's address, size or type is another."""
+        ts = self.tensors
+        key = (list(map(_data_ptr, ts)), list(map(_numel, ts)), [t.dtype for t in ts])
         if key != self._key:
-            arr = (_lib.TensorItem * max(1, len(self.tensors)))()
-            for it, t in zip(arr, self.tensors):
+            arr = (_lib.TensorItem * max(1, len(ts)))()
+            for it, t in zip(arr, ts):
                 if t.numel() and not _is_dense(t):
                     raise ValueError("hsidm: a gradient of shape %s with strides %s is not dense" % (tuple(t.shape), t.stride()))
                 it.ptr, it.n, it.type = t.data_ptr(), t.numel(), _lib.type_id(t.dtype)
-            spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.tensors if t.numel())
+            spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts if t.numel())
             self._disjoint = all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
             self._items, self._key = arr, key
         return self._items
@@ -367,13 +373,13 @@ def clip_grad_norm_(tensors, max_norm):
 def qk_norm_rope_bwd(d_out_q, d_out_k, q, k, wq, wk, pos, axes, eps=1e-6, out=None):
     """Gradient of ops.qk_norm_rope: (dq, dk, dwq, dwk) from the gradients of its two results and its inputs; dq / dk in the inputs'
     type, dwq / dwk fp32 [D].  out: optional (dq, dk) to write into, [T, H, D] views with 16-byte aligned rows (slices of a dqkv)."""
-    d, keep = ops.rope_desc(q, k, wq, wk, pos, axes, eps)
+    d, nb, keep = ops.rope_desc(q, k, wq, wk, pos, axes, eps)
     T, D = q.shape[0], q.shape[2]
     for g, x in ((d_out_q, q), (d_out_k, k)):
         if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
             raise ValueError("hsidm: a gradient of %s %s does not belong to a tensor of %s %s" % (tuple(g.shape), g.dtype, tuple(x.shape), x.dtype))
-    dq, dk = (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)) if out is None else out
-    for g, x in ((dq, q), (dk, k)):
+    dq, dk = (q.new_empty(q.shape), k.new_empty(k.shape)) if out is None else out
+    for g, x in () if out is None else ((dq, q), (dk, k)):
         if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device or not ops.rows_aligned(g):
             raise ValueError("hsidm: out must be [T, H, D] tensors like q and k with 16-byte aligned rows")
     dwq, dwk = (torch.zeros if T == 0 else torch.empty)((2, D), dtype=torch.float32, device=q.device).unbind(0)
@@ -381,29 +387,29 @@ def qk_norm_rope_bwd(d_out_q, d_out_k, q, k, wq, wk, pos, axes, eps=1e-6, out=No
         return dq, dk, dwq, dwk
     L = _lib.lib()
     with _lib.on_device(q.device):
-        nb = L.hsidm_qk_norm_rope_bwd_workspace_bytes(C.byref(d))
-        if nb < 0:
-            _check(int(nb), "qk_norm_rope_bwd_workspace_bytes")
-        ws = torch.empty(int(nb), dtype=torch.uint8, device=q.device)
-        gq, gk = d_out_q.contiguous(), d_out_k.contiguous()
-        _check(L.hsidm_qk_norm_rope_bwd(C.byref(d), ops.base(gq), ops.base(gk), ops.base(dq), dq.stride(0), dq.stride(1), ops.base(dk), dk.stride(0),
-                                        dk.stride(1), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), int(nb), _lib.stream_ptr()), "qk_norm_rope_bwd")
+        ws = q.new_empty(nb, dtype=torch.uint8)
+        gq, gk = ops._aligned(d_out_q), ops._aligned(d_out_k)
+        _check(L.hsidm_qk_norm_rope_bwd(C.byref(d), gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0),
+                                        dk.stride(1), dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), nb, _lib.stream_ptr()), "qk_norm_rope_bwd")
     return dq, dk, dwq, dwk
 
 
-def attention_packed_bwd(do, q, k, v, out, lse, seqs, causal=False, scale=None, grads=None):
-    """Gradient of ops.attention_packed: (dq, dk, dv) in the inputs' type from the output's gradient do, the inputs, the output and its lse.
-    grads: optional (dq, dk, dv) to write into, [T, H, D] views with 16-byte aligned rows (slices of a dqkv)."""
-    d, keep = ops.attn_desc(q, k, v, seqs, causal, scale)
+def attention_packed_bwd(do, q, k, v, out, saved, seqs, causal=False, scale=None, grads=None):
+    """Gradient of ops.attention_packed: (dq, dk, dv) in the inputs' type from the output's gradient do, the inputs, the output and what
+    the forward pass saved (its AttentionSaved).  grads: optional (dq, dk, dv) to write into, [T, H, D] views with 16-byte aligned rows
+    (slices of a dqkv)."""
+    d, _, nb, keep = ops.attn_desc(q, k, v, seqs, causal, scale)
     T, Hq, _ = q.shape
-    for t in (do, out):
+    lse, lo = saved
+    for t in (do, out) + (() if lo is None else (lo,)):
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
-            raise ValueError("hsidm: do and out must be like q: %s %s, got %s %s" % (tuple(q.shape), q.dtype, tuple(t.shape), t.dtype))
+            raise ValueError("hsidm: do, out and its residual must be like q: %s %s, got %s %s" % (tuple(q.shape), q.dtype, tuple(t.shape), t.dtype))
     if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or lse.device != q.device:
         raise ValueError("hsidm: lse must be attention_packed's fp32 [%d, %d], got %s %s" % (Hq, T, lse.dtype, tuple(lse.shape)))
-    if grads is None:
-        grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    for g, x in zip(grads, (q, k, v)):
+    own = grads is None
+    if own:
+        grads = (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape))
+    for g, x in () if own else zip(grads, (q, k, v)):
         if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device or not ops.rows_aligned(g):
             raise ValueError("hsidm: grads must be [T, H, D] tensors like q, k, v with 16-byte aligned rows")
     dq, dk, dv = grads
@@ -411,14 +417,12 @@ def attention_packed_bwd(do, q, k, v, out, lse, seqs, causal=False, scale=None, 
         return dq, dk, dv
     L = _lib.lib()
     with _lib.on_device(q.device):
-        nb = L.hsidm_attention_packed_bwd_workspace_bytes(C.byref(d))
-        if nb < 0:
-            _check(int(nb), "attention_packed_bwd_workspace_bytes")
-        ws = torch.empty(int(nb), dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(nb, dtype=torch.uint8)
         do, out, lse = ops.token_rows(do), ops._aligned(out), lse.contiguous()
+        lo = None if lo is None else ops._aligned(lo)
         args = []
         for t in (do, dq, dk, dv):
             args += [t.data_ptr(), *ops._strides(t)]
-        _check(L.hsidm_attention_packed_bwd(C.byref(d), out.data_ptr(), _lib.ptr(lse), *args, _lib.ptr(ws), int(nb), _lib.stream_ptr()),
+        _check(L.hsidm_attention_packed_bwd(C.byref(d), out.data_ptr(), _lib.ptr(lo), lse.data_ptr(), *args, ws.data_ptr(), nb, _lib.stream_ptr()),
                "attention_packed_bwd")
     return dq, dk, dv

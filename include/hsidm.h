@@ -232,7 +232,9 @@ int hsidm_attention(int prec, const void* qkv, void* out, int B, int N, int C, v
  * order query tiles should start (most work first), ktiles: key tiles.  longest: the longest sequence.  Rows that no tile covers are not
  * written.
  * Values of k and v must be finite where a LATER token of the same 128-row tile is masked out for an earlier one (0 * inf is NaN).
- * Backward: from out, lse and dout, recomputing the scores: dq, dk, dv (strided like their tensors), dk / dv summed over the heads that
+ * out_lo (16-bit types; may be NULL): what rounding out to the type left behind, for the backward pass: rowsum(dout o out) from both is
+ *   exact to fp32, and dq / dk are then as exact as rounding dS allows.
+ * Backward: from out (+ out_lo), lse and dout, recomputing the scores: dq, dk, dv (strided like their tensors), dk / dv summed over the heads that
  * share them; no atomics, fixed order.  Workspaces: the _workspace_bytes functions (forward: 0 unless the keys are split), 16-byte aligned. */
 typedef struct hsidm_attn_tile { int32_t start, len, row0, reserved; } hsidm_attn_tile;
 typedef struct hsidm_attn_desc {
@@ -240,15 +242,16 @@ typedef struct hsidm_attn_desc {
     int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
     int64_t T;
     const hsidm_attn_tile *qtiles64, *qtiles128, *ktiles64, *ktiles128;
+    double pairs;                            /* (query, key) pairs of one head: sum of len^2, causal len (len + 1) / 2 */
     int32_t n64, n128, longest;
     int32_t Hq, Hk, D, prec, causal;
     float scale;
 } hsidm_attn_desc;
 int64_t hsidm_attention_packed_workspace_bytes(const hsidm_attn_desc* d);
-int hsidm_attention_packed(const hsidm_attn_desc* d, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int hsidm_attention_packed(const hsidm_attn_desc* d, void* out, void* out_lo, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t hsidm_attention_packed_bwd_workspace_bytes(const hsidm_attn_desc* d);
-int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* out, const float* lse, const void* dout, int64_t do_ts, int64_t do_hs,
-                               void* dq, int64_t dq_ts, int64_t dq_hs, void* dk, int64_t dk_ts, int64_t dk_hs, void* dv, int64_t dv_ts,
+int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* out, const void* out_lo, const float* lse, const void* dout, int64_t do_ts,
+                               int64_t do_hs, void* dq, int64_t dq_ts, int64_t dq_hs, void* dk, int64_t dk_ts, int64_t dk_hs, void* dv, int64_t dv_ts,
                                int64_t dv_hs, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- RMS norm of queries and keys per head + rotation by positions with several axes, one pass -------------------------------

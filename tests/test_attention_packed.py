@@ -117,7 +117,7 @@ def test_refusals_without_a_gpu():
     def desc(**kw):
         d = _lib.AttnDesc()
         vals = dict(q=64, k=64, v=64, q_ts=256, q_hs=64, k_ts=128, k_hs=64, v_ts=128, v_hs=64, T=10, qtiles64=64, qtiles128=64, ktiles64=64, ktiles128=64,
-                    n64=2, n128=2, longest=6, Hq=4, Hk=2, D=64, prec=_lib.BF16, causal=1, scale=0.125)
+                    n64=2, n128=2, longest=6, pairs=31.0, Hq=4, Hk=2, D=64, prec=_lib.BF16, causal=1, scale=0.125)
         for n, v in {**vals, **kw}.items():
             setattr(d, n, v)
         return ctypes.byref(d)
@@ -126,16 +126,16 @@ def test_refusals_without_a_gpu():
     need = L.hsidm_attention_packed_bwd_workspace_bytes(desc())
     assert need > 10 * 4 * 4
     for bad in (dict(T=0), dict(Hk=3), dict(Hk=0), dict(D=0), dict(D=260), dict(D=36), dict(prec=5), dict(scale=0.0), dict(scale=math.nan), dict(q=72),
-                dict(k_hs=4), dict(v_ts=-64), dict(n64=0), dict(longest=0), dict(qtiles64=None), dict(ktiles128=None)):
+                dict(k_hs=4), dict(v_ts=-64), dict(n64=0), dict(longest=0), dict(pairs=0.0), dict(pairs=math.nan), dict(qtiles64=None), dict(ktiles128=None)):
         assert L.hsidm_attention_packed_workspace_bytes(desc(**bad)) == -1, bad
-        assert L.hsidm_attention_packed(desc(**bad), one, one, one, 1 << 30, None) == -1, bad
-        assert L.hsidm_attention_packed_bwd(desc(**bad), one, one, *[one, 256, 64] * 4, one, 1 << 30, None) == -1, bad
-    assert L.hsidm_attention_packed(None, one, one, one, 0, None) == -1
-    assert L.hsidm_attention_packed(desc(), None, one, one, 1 << 30, None) == -1
-    assert L.hsidm_attention_packed(desc(longest=100000), one, one, one, 0, None) == -1          # the split form without its workspace
-    assert L.hsidm_attention_packed_bwd(desc(), one, one, *[one, 256, 64] * 4, one, need - 1, None) == -1
-    assert L.hsidm_attention_packed_bwd(desc(), one, None, *[one, 256, 64] * 4, one, need, None) == -1
-    assert L.hsidm_attention_packed_bwd(desc(), one, one, *[one, 256, 63] * 4, one, need, None) == -1
+        assert L.hsidm_attention_packed(desc(**bad), one, None, one, one, 1 << 30, None) == -1, bad
+        assert L.hsidm_attention_packed_bwd(desc(**bad), one, None, one, *[one, 256, 64] * 4, one, 1 << 30, None) == -1, bad
+    assert L.hsidm_attention_packed(None, one, None, one, one, 0, None) == -1
+    assert L.hsidm_attention_packed(desc(), None, None, one, one, 1 << 30, None) == -1
+    assert L.hsidm_attention_packed(desc(longest=100000), one, None, one, one, 0, None) == -1          # the split form without its workspace
+    assert L.hsidm_attention_packed_bwd(desc(), one, None, one, *[one, 256, 64] * 4, one, need - 1, None) == -1
+    assert L.hsidm_attention_packed_bwd(desc(), one, None, None, *[one, 256, 64] * 4, one, need, None) == -1
+    assert L.hsidm_attention_packed_bwd(desc(), one, None, one, *[one, 256, 63] * 4, one, need, None) == -1
 
 
 # ------------------------------------------------------------------------------------------------------------------- GPU
@@ -158,13 +158,25 @@ def test_forward_and_backward(dev, case, kind):
     q, k, v, do = make(dev, lengths, hq, hk, D, dtype)
     seqs = ops.PackedSequences(lengths, device=dev)
     scale = D ** -0.5
-    o, lse = ops.attention_packed(q, k, v, seqs, causal=causal, want_lse=True)
+    o, saved = ops.attention_packed(q, k, v, seqs, causal=causal, want_lse=True)
     assert torch.equal(o, ops.attention_packed(q, k, v, seqs, causal=causal))
     want, want_lse = plain64(q, k, v, lengths, causal, scale, do)
     close(o, want["o"], want["mo"], 2, "out")
-    assert float((lse.double() - want_lse).abs().max()) <= SCORES * 2.0 ** -24 * 2
-    grads = Tr.attention_packed_bwd(do, q, k, v, o, lse, seqs, causal=causal)
-    again = Tr.attention_packed_bwd(do, q, k, v, o, lse, seqs, causal=causal)
+    assert float((saved.lse.double() - want_lse).abs().max()) <= SCORES * 2.0 ** -24 * 2
+    # (the residual is what the fp32 output lost in the store: together they are within a step of the residual's own rounding, fp32's errors
+    # and the probabilities' rounding)
+    assert (saved.residual is None) == (kind == "fp32")
+    if saved.residual is not None:
+        u = torch.finfo(dtype).eps / 2
+        both = o.double() + saved.residual.double()
+        tol = want["o"].abs() * u * u * 4 + want["mo"] * (2 * u + SCORES * 2.0 ** -24) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert bool(((both - want["o"]).abs() <= tol).all())
+        assert bool((saved.residual.double().abs() <= o.double().abs() * 2 * u + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps).all())
+    grads = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, causal=causal)
+    bare = Tr.attention_packed_bwd(do, q, k, v, o, (saved.lse, None), seqs, causal=causal)
+    for name, g in zip(("dq", "dk", "dv"), bare):
+        close(g, want[name], want["m" + name], 4, name + " without the residual")
+    again = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, causal=causal)
     for name, g, a in zip(("dq", "dk", "dv"), grads, again):
         assert torch.equal(g, a), name
         close(g, want[name], want["m" + name], 4, name)
@@ -183,8 +195,8 @@ def test_long_rows_and_gradient_sizes(dev, kind, do_gain):
     q, k, v, do = make(dev, lengths, 2, 1, 64, dtype, seed=2, gain=0.5)
     do = (do.float() * do_gain).to(dtype)
     seqs = ops.PackedSequences(lengths, device=dev)
-    o, lse = ops.attention_packed(q, k, v, seqs, want_lse=True)
-    got = Tr.attention_packed_bwd(do, q, k, v, o, lse, seqs)
+    o, saved = ops.attention_packed(q, k, v, seqs, want_lse=True)
+    got = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs)
     want, _ = plain64(q, k, v, lengths, False, 0.125, do)
     u = torch.finfo(dtype).eps / 2
     for name, g in zip(("o", "dq", "dk", "dv"), (o,) + got):
@@ -210,12 +222,12 @@ def test_large_scores_and_lazy_maximum(dev):
         qq = (q * 0.1 + torch.ones(1, 1, D)).to(dev)
         seqs = ops.PackedSequences([T], device=dev)
         for causal in (False, True):
-            o, lse = ops.attention_packed(qq, kk, v, seqs, causal=causal, scale=1.0, want_lse=True)
+            o, saved = ops.attention_packed(qq, kk, v, seqs, causal=causal, scale=1.0, want_lse=True)
             want, want_lse = plain64(qq, kk, v, [T], causal, 1.0)
             # scores up to 400: an fp32 score is off by 400 * 2^-24 * sqrt(D)
             tol = 2.0 ** -24 * (gain + 8) * 16
             assert float((o.double() - want["o"]).abs().max()) <= tol * 8
-            assert float((lse.double() - want_lse).abs().max()) <= tol * 8
+            assert float((saved.lse.double() - want_lse).abs().max()) <= tol * 8
 
 
 @GPU
@@ -227,8 +239,8 @@ def test_values_of_other_sequences_never_matter(dev):
     for dtype in TYPES.values():
         q, k, v, do = make(dev, lengths, 2, 1, 64, dtype, seed=4)
         seqs = ops.PackedSequences(lengths, device=dev)
-        o, lse = ops.attention_packed(q, k, v, seqs, causal=True, want_lse=True)
-        g = Tr.attention_packed_bwd(do, q, k, v, o, lse, seqs, causal=True)
+        o, saved = ops.attention_packed(q, k, v, seqs, causal=True, want_lse=True)
+        g = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, causal=True)
         for bad in (math.nan, math.inf):
             qb, kb, vb, db = q.clone(), k.clone(), v.clone(), do.clone()
             for x in (qb, kb, vb, db):
@@ -260,20 +272,20 @@ def test_layouts(dev, layout):
                "expanded": lambda: [t[:, :1].expand(T, H, D) for t in qkv.view(T, 3, H, D).unbind(1)]}[layout]()
     seqs = ops.PackedSequences(lengths, device=dev)
     dense = [t.clone(memory_format=torch.contiguous_format) for t in (q, k, v)]
-    o, lse = ops.attention_packed(q, k, v, seqs, want_lse=True)
+    o, saved = ops.attention_packed(q, k, v, seqs, want_lse=True)
     o2, lse2 = ops.attention_packed(*dense, seqs, want_lse=True)
-    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    assert torch.equal(o, o2) and torch.equal(saved.lse, lse2.lse) and torch.equal(saved.residual, lse2.residual)
     do = torch.randn(T, H, 2 * D, device=dev).to(dtype)[..., ::2]
     views = (grads[:, 0:H], grads[:, H:2 * H], grads[:, 2 * H:3 * H])
-    got = Tr.attention_packed_bwd(do, q, k, v, o, lse, seqs, grads=views)
+    got = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, grads=views)
     want = Tr.attention_packed_bwd(do.contiguous(), *dense, o2, lse2, seqs)
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and bool((grads[:, 3 * H] == 9).all())
     with pytest.raises(ValueError, match="grads"):
-        Tr.attention_packed_bwd(do, q, k, v, o, lse, seqs, grads=(views[0], views[1], views[2].float()))
+        Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, grads=(views[0], views[1], views[2].float()))
     with pytest.raises(ValueError, match="lse"):
-        Tr.attention_packed_bwd(do, q, k, v, o, lse[:, :-1], seqs)
+        Tr.attention_packed_bwd(do, q, k, v, o, (saved.lse[:, :-1], None), seqs)
     with pytest.raises(ValueError, match="like q"):
-        Tr.attention_packed_bwd(do[:-1], q, k, v, o, lse, seqs)
+        Tr.attention_packed_bwd(do[:-1], q, k, v, o, saved, seqs)
 
 
 @GPU
@@ -283,9 +295,9 @@ def test_no_tokens(dev):
     for lengths in ([], [0, 0]):
         seqs = ops.PackedSequences(lengths, device=dev)
         e = torch.empty(0, 2, 64, device=dev)
-        o, lse = ops.attention_packed(e, e, e, seqs, want_lse=True)
-        assert o.shape == e.shape and lse.shape == (2, 0)
-        assert all(g.shape == e.shape for g in Tr.attention_packed_bwd(e, e, e, e, o, lse, seqs))
+        o, saved = ops.attention_packed(e, e, e, seqs, want_lse=True)
+        assert o.shape == e.shape and saved.lse.shape == (2, 0)
+        assert all(g.shape == e.shape for g in Tr.attention_packed_bwd(e, e, e, e, o, saved, seqs))
 
 
 @GPU
@@ -295,8 +307,8 @@ def test_gradient_against_differences(dev):
     lengths = [37, 70]
     q, k, v, do = make(dev, lengths, 4, 2, 32, torch.float32, seed=6)
     seqs = ops.PackedSequences(lengths, device=dev)
-    o, lse = ops.attention_packed(q, k, v, seqs, causal=True, want_lse=True)
-    grads = Tr.attention_packed_bwd(do, q, k, v, o, lse, seqs, causal=True)
+    o, saved = ops.attention_packed(q, k, v, seqs, causal=True, want_lse=True)
+    grads = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, causal=True)
     g = torch.Generator().manual_seed(1)
     for i, gx in enumerate(grads):
         x = [q, k, v]
@@ -317,8 +329,8 @@ def test_captured_and_on_another_stream(dev, lengths):
     seqs = ops.PackedSequences(lengths, device=dev)
 
     def step():
-        o, lse = ops.attention_packed(q, k, v, seqs, causal=True, want_lse=True)
-        return (o, lse) + Tr.attention_packed_bwd(do, q, k, v, o, lse, seqs, causal=True)
+        o, saved = ops.attention_packed(q, k, v, seqs, causal=True, want_lse=True)
+        return (o, saved.lse, saved.residual) + Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, causal=True)
     step()
     torch.cuda.synchronize()
     graphs = []
