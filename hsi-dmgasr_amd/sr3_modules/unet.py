@@ -248,15 +248,61 @@ class ResnetBlock(_HipModule):
 
 
 class SelfAttention(_HipModule):
-    def __init__(self, in_channel, n_head=1, norm_groups=32):
+    """Reference unet.py:114-143.  Maps of more than 1024 tokens - the reference's own einsum has no limit - run on the packed attention
+    kernels (ops.attention_packed), which store nothing of size tokens^2; heads up to 256 channels there.
+
+    qk_norm_rope (not in the reference; default off): queries and keys of every head pass an RMS norm (weights q_norm, k_norm) and are
+    rotated by their pixel's row and column, half of the pairs each (ops.qk_norm_rope) - the only position information in the layer."""
+
+    def __init__(self, in_channel, n_head=1, norm_groups=32, *, qk_norm_rope=False):
         super().__init__()
         if in_channel % n_head:
             raise ValueError("in_channel must be a multiple of n_head")
         self.n_head = n_head
+        self.qk_norm_rope = bool(qk_norm_rope)
+        if self.qk_norm_rope:
+            dim = in_channel // n_head
+            if dim % 16 or dim > 256:
+                raise ValueError("hsidm: qk_norm_rope needs heads of a multiple of 16 channels up to 256, got %d" % dim)
+            self.q_norm, self.k_norm = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.ones(dim))
         self.norm = nn.GroupNorm(norm_groups, in_channel)
         self.qkv = nn.Conv2d(in_channel, in_channel * 3, 1, bias=False)
         self.out = nn.Conv2d(in_channel, in_channel, 1)
         self._cache = _PackCache()
+        self._maps = {}
+
+    def packed(self, tokens):
+        """Does a map of that many tokens run on the packed attention kernels?"""
+        return self.qk_norm_rope or tokens > 1024
+
+    def map_plan(self, B, H, W, device):
+        """(sequences, positions, axes) of a batch of maps, kept per shape for good (captured steps hold their addresses; about nine bytes
+        a token): one sequence per image; (row, column) of every token."""
+        key = (B, H, W, device)
+        plan = self._maps.get(key)
+        if plan is None:
+            seqs, pos, axes = ops.PackedSequences([H * W] * B, device=device), None, None
+            if self.qk_norm_rope:
+                grid = torch.stack(torch.meshgrid(torch.arange(H, dtype=torch.int32), torch.arange(W, dtype=torch.int32), indexing="ij"), dim=-1)
+                pos = grid.reshape(1, H * W, 2).expand(B, -1, -1).reshape(-1, 2).contiguous().to(device)
+                dim = self.q_norm.shape[0]
+                axes = ops.RotaryAxes((dim // 4, dim // 4), dim, device=device)
+            plan = self._maps[key] = (seqs, pos, axes)
+        return plan
+
+    def heads(self, qkv):
+        """(q, k, v) [tokens, n_head, head channels] as views of the qkv projection's output (reference unet.py:131-132: head by head,
+        q | k | v within a head)."""
+        B, H, W, C3 = qkv.shape
+        return qkv.view(B * H * W, self.n_head, 3, C3 // (3 * self.n_head)).unbind(2)
+
+    def _packed_core(self, qkv):
+        B, H, W, C3 = qkv.shape
+        seqs, pos, axes = self.map_plan(B, H, W, qkv.device)
+        q, k, v = self.heads(qkv)
+        if self.qk_norm_rope:
+            q, k = ops.qk_norm_rope(q, k, self.q_norm.detach(), self.k_norm.detach(), pos, axes)
+        return ops.attention_packed(q, k, v, seqs, scale=(C3 // 3) ** -0.5).view(B, H, W, C3 // 3)
 
     def _run(self, x, precision):
         pq = self._cache.get(("qkv", precision), [self.qkv.weight], lambda: ops.PackedConv(self.qkv.weight, None, precision))
@@ -266,7 +312,10 @@ class SelfAttention(_HipModule):
         qkv = ops.conv2d(x, pq, gn_ab=ab, transform=ops.XF_AFFINE)
         # (the reference's UNet only ever builds n_head = 1, unet.py:152: the fused MFMA kernel; more heads go through the
         # strided GEMM + softmax kernels)
-        o = ops.attention(qkv, precision) if self.n_head == 1 else ops.attention_multihead(qkv, self.n_head, precision)
+        if self.packed(x.shape[1] * x.shape[2]):
+            o = self._packed_core(qkv)
+        else:
+            o = ops.attention(qkv, precision) if self.n_head == 1 else ops.attention_multihead(qkv, self.n_head, precision)
         return ops.conv2d(o, po, res=x, stats=True)
 
     def forward(self, input):
@@ -276,12 +325,12 @@ class SelfAttention(_HipModule):
 
 
 class ResnetBlocWithAttn(_HipModule):
-    def __init__(self, dim, dim_out, *, noise_level_emb_dim=None, norm_groups=32, dropout=0, with_attn=False):
+    def __init__(self, dim, dim_out, *, noise_level_emb_dim=None, norm_groups=32, dropout=0, with_attn=False, qk_norm_rope=False):
         super().__init__()
         self.with_attn = with_attn
         self.res_block = ResnetBlock(dim, dim_out, noise_level_emb_dim, norm_groups=norm_groups, dropout=dropout)
         if with_attn:
-            self.attn = SelfAttention(dim_out, norm_groups=norm_groups)
+            self.attn = SelfAttention(dim_out, norm_groups=norm_groups, qk_norm_rope=qk_norm_rope)
 
     def _run(self, x0, x1, film, precision):
         x = self.res_block._run(x0, x1, film, precision)
@@ -298,7 +347,7 @@ class ResnetBlocWithAttn(_HipModule):
 
 class UNet(_HipModule):
     def __init__(self, in_channel=6, out_channel=3, inner_channel=32, norm_groups=32, channel_mults=(1, 2, 4, 8, 8),
-                 attn_res=(8), res_blocks=3, dropout=0, with_noise_level_emb=True, image_size=128, precision=None):
+                 attn_res=(8), res_blocks=3, dropout=0, with_noise_level_emb=True, image_size=128, precision=None, attn_qk_norm_rope=False):
         super().__init__()
         if not with_noise_level_emb:
             # the reference cannot build this variant either: its ResnetBlock constructs nn.Linear(None, dim_out)
@@ -319,7 +368,7 @@ class UNet(_HipModule):
 
         def unit(cin, cout, attn):
             return ResnetBlocWithAttn(cin, cout, noise_level_emb_dim=emb, norm_groups=norm_groups, dropout=dropout,
-                                      with_attn=attn)
+                                      with_attn=attn, qk_norm_rope=attn_qk_norm_rope)
 
         # encoder: stem conv, then per level `res_blocks` units (+ a stride-2 conv between levels)
         width = inner_channel

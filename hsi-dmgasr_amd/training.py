@@ -343,16 +343,46 @@ class Trainer:
         ab = ops.gn_scale_shift(x, None, at.norm.weight, at.norm.bias, at.norm.num_groups, p, at.norm.eps)
         n = T.gn_act_apply(x, None, ab, False, p)
         qkv = ops.conv2d(n, self.pk(at.qkv))
-        o = ops.attention(qkv, p)
+        if at.packed(x.shape[1] * x.shape[2]):
+            o, core = self._packed_attn_fwd(at, qkv)
+        else:
+            o, core = ops.attention(qkv, p), None
         y = ops.conv2d(o, self.pk(at.out), res=x, stats=True)
-        return y, (x, ab, n, qkv, o)
+        return y, (x, ab, n, qkv, o, core)
+
+    def _packed_attn_fwd(self, at, qkv):
+        """The attention core of a layer that runs on packed sequences: output and what its backward needs."""
+        B, H, W, C3 = qkv.shape
+        seqs, pos, axes = at.map_plan(B, H, W, qkv.device)
+        q, k, v = at.heads(qkv)
+        if at.qk_norm_rope:
+            q, k = ops.qk_norm_rope(q, k, at.q_norm.detach(), at.k_norm.detach(), pos, axes)
+        o, saved = ops.attention_packed(q, k, v, seqs, scale=(C3 // 3) ** -0.5, want_lse=True)
+        return o.view(B, H, W, C3 // 3), (q, k, saved)
+
+    def _packed_attn_bwd(self, at, qkv, o, do, core):
+        """Gradient of _packed_attn_fwd at its qkv; q_norm's and k_norm's go to the gradient buffer."""
+        B, H, W, C3 = qkv.shape
+        seqs, pos, axes = at.map_plan(B, H, W, qkv.device)
+        q, k, saved = core
+        q0, k0, v = at.heads(qkv)
+        dqkv = torch.empty_like(qkv)
+        dq, dk, dv = at.heads(dqkv)
+        rope = at.qk_norm_rope
+        into = (torch.empty_like(q), torch.empty_like(k), dv) if rope else (dq, dk, dv)
+        T.attention_packed_bwd(do.view(q.shape), q, k, v, o.view(q.shape), saved, seqs, scale=(C3 // 3) ** -0.5, grads=into)
+        if rope:
+            _, _, dwq, dwk = T.qk_norm_rope_bwd(into[0], into[1], q0, k0, at.q_norm.detach(), at.k_norm.detach(), pos, axes, out=(dq, dk))
+            self.G(at.q_norm).copy_(dwq)
+            self.G(at.k_norm).copy_(dwk)
+        return dqkv
 
     def _attn_bwd(self, at, ctx, dy):
-        x, ab, n, qkv, o = ctx
+        x, ab, n, qkv, o, core = ctx
         p = self.precision
         T.conv_wgrad(o, None, dy, self.G(at.out.weight), p, deferred=self._defer, db=self.G(at.out.bias))
         do = ops.conv2d(dy, self.dpk(at.out))
-        dqkv = T.attention_bwd(qkv, do, p)
+        dqkv = T.attention_bwd(qkv, do, p) if core is None else self._packed_attn_bwd(at, qkv, o, do, core)
         T.conv_wgrad(n, None, dqkv, self.G(at.qkv.weight), p, deferred=self._defer)
         dn = ops.conv2d(dqkv, self.dpk(at.qkv))
         dx, _ = T.gn_act_bwd(dn, x, None, ab, at.norm.weight, at.norm.num_groups, False, p, self.G(at.norm.weight),
