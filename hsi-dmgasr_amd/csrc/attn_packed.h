@@ -51,23 +51,39 @@ template <typename T, int DP> struct Row {
 };
 
 // Requests rows [row0, row0 + ROWS) of a sequence (clamped to its last) into an LDS tile: every wave of the workgroup takes its share of
-// 1 KB instructions.  base: the sequence's first row, this head.  Complete after wait_loads() and a barrier.
-template <typename T, int DP, int ROWS, int NW>
-__device__ __forceinline__ void stage_rows(const char* base, int64_t ts, int row0, int len, int pieces, char* tile, int wave, int lane) {
+// 1 KB instructions.  base: the sequence's first row, this head.  Complete after wait_loads() and a barrier.  A lane's place among the
+// rows is a 32-bit offset made once; what moves from tile to tile and from instruction to instruction is a scalar base, so that a whole
+// tile costs the vector unit nothing (with 64-bit addresses per lane it was a quarter of its work at D = 64).
+template <typename T, int DP, int ROWS, int NW> struct Stage {
     typedef Row<T, DP> R;
-    constexpr int PER_WAVE = ROWS * R::PIECES / 64 / NW;
-    static_assert(ROWS * R::PIECES % (64 * NW) == 0, "a tile is whole instructions of every wave");
+    static constexpr int PER_WAVE = ROWS * R::PIECES / 64 / NW, STEP = NW * 64 / R::PIECES;      // STEP: rows from one instruction to the next
+    static constexpr int PAT = STEP % 8 == 0 ? 1 : 8 / STEP;         // instructions until the exchange of pieces repeats
+    static_assert(ROWS * R::PIECES % (64 * NW) == 0 && (STEP % 8 == 0 || 8 % STEP == 0), "a tile is whole instructions of every wave");
+    uint32_t off[PAT], ts;
+    int r0;
+    __device__ __forceinline__ Stage(int64_t token_stride, int pieces, int wave, int lane) : ts((uint32_t)token_stride) {
+        const int idx = wave * 64 + lane;
+        r0 = idx / R::PIECES;
 #pragma unroll
-    for (int i = 0; i < PER_WAVE; ++i) {
-        const int first = (i * NW + wave) * 64, idx = first + lane, r = idx / R::PIECES;
-        int c = (idx % R::PIECES) ^ R::swz(r);
-        c = c < pieces ? c : pieces - 1;
-        int g = row0 + r;
-        g = g < len ? g : len - 1;
-        const char* src = base + (int64_t)g * ts + c * 16;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)(tile + first * 16), 16, 0, 0);
+        for (int x = 0; x < PAT; ++x) off[x] = (uint32_t)r0 * ts + (uint32_t)min((idx % R::PIECES) ^ R::swz(r0 + x * STEP), pieces - 1) * 16u;
     }
-}
+    __device__ __forceinline__ void operator()(const char* base, int row0, int len, char* tile, int wave) const {
+        if (row0 + ROWS <= len) {
+#pragma unroll
+            for (int i = 0; i < PER_WAVE; ++i) load(base + (int64_t)(row0 + i * STEP) * ts, off[i % PAT], tile, wave, i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER_WAVE; ++i) {
+                const int g = min(row0 + r0 + i * STEP, len - 1) - row0;             // (row0 < len: the tile has a row)
+                load(base + (int64_t)row0 * ts, off[i % PAT] + (uint32_t)(g - r0) * ts, tile, wave, i);
+            }
+        }
+    }
+    static __device__ __forceinline__ void load(const char* base, uint32_t offset, char* tile, int wave, int i) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + offset),
+                                         (__attribute__((address_space(3))) void*)(tile + (i * NW + wave) * 1024), 16, 0, 0);
+    }
+};
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // a row of a sequence in registers, as the row operand of every step: zero beyond D
@@ -250,9 +266,10 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
     const Places<T, DP> at(lane);
     const float c = a.scale * kLog2e;
     float m = -INFINITY, l = 0.f;                                    // m: the scaling maximum in score units; l: this half's share of the sum
+    const Stage<T, DP, BN, NW> kst(a.k.ts, pieces, wave, lane), vst(a.v.ts, pieces, wave, lane);
     auto stage = [&](int t, int buf) __attribute__((always_inline)) {
-        stage_rows<T, DP, BN, NW>(kb, a.k.ts, t * BN, len, pieces, lds + buf * 2 * TILE, wave, lane);
-        stage_rows<T, DP, BN, NW>(vb, a.v.ts, t * BN, len, pieces, lds + buf * 2 * TILE + TILE, wave, lane);
+        kst(kb, t * BN, len, lds + buf * 2 * TILE, wave);
+        vst(vb, t * BN, len, lds + buf * 2 * TILE + TILE, wave);
     };
     if (t0 < t1) stage(t0, 0);
     wait_loads();
@@ -374,7 +391,7 @@ template <typename T> __device__ __forceinline__ void store_grad(const AttnTenso
 template <typename T, int DP> struct KvTiles { static constexpr int ND = DP > 128 ? DP / 64 : DP / 32, PARTS = DP / 32 / ND; };
 
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 128 ? 2 : 1)) void attn_bwd_kv_kernel(AttnBwdArgs a) {
+__global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_bwd_kv_kernel(AttnBwdArgs a) {
     typedef Row<T, DP> R;
     constexpr int BQ = R::BYTES <= 256 ? 64 : 32, ND = KvTiles<T, DP>::ND, TILE = BQ * R::BYTES, BUF = 2 * TILE + 512;
     extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][Q tile, dO tile, lse[64], delta[64]]
@@ -398,11 +415,12 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 128 ? 2 : 1)) void a
     const float c = a.scale * kLog2e;
     float f = 1.f;
     if constexpr (GradScale<T>::on) f = grad_factor(a.maxima, a.nmax, lane);
+    const Stage<T, DP, BQ, NW> qst(a.q.ts, pieces, wave, lane), gst(a.dout.ts, pieces, wave, lane);
     auto stage = [&](int w, int buf) __attribute__((always_inline)) {
         const int g = w / ntq, t = tq0 + w - g * ntq, head = kvh * group + g;
         char* b = lds + buf * BUF;
-        stage_rows<T, DP, BQ, NW>(a.q.p + (int64_t)tile.start * a.q.ts + head * a.q.hs, a.q.ts, t * BQ, len, pieces, b, wave, lane);
-        stage_rows<T, DP, BQ, NW>(a.dout.p + (int64_t)tile.start * a.dout.ts + head * a.dout.hs, a.dout.ts, t * BQ, len, pieces, b + TILE, wave, lane);
+        qst(a.q.p + (int64_t)tile.start * a.q.ts + head * a.q.hs, t * BQ, len, b, wave);
+        gst(a.dout.p + (int64_t)tile.start * a.dout.ts + head * a.dout.hs, t * BQ, len, b + TILE, wave);
         if (wave < 2) {                                              // 64 floats each; rows past the tile are not read back
             const float* src = (wave == 0 ? a.lse : a.delta) + head * a.T + tile.start + min(t * BQ + lane, len - 1);
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
@@ -512,9 +530,10 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
     const float c = a.scale * kLog2e;
     float f = 1.f;
     if constexpr (GradScale<T>::on) f = grad_factor(a.maxima, a.nmax, lane);
+    const Stage<T, DP, BN, NW> kst(a.k.ts, pieces, wave, lane), vst(a.v.ts, pieces, wave, lane);
     auto stage = [&](int t, int buf) __attribute__((always_inline)) {
-        stage_rows<T, DP, BN, NW>(kb, a.k.ts, t * BN, len, pieces, lds + buf * 2 * TILE, wave, lane);
-        stage_rows<T, DP, BN, NW>(vb, a.v.ts, t * BN, len, pieces, lds + buf * 2 * TILE + TILE, wave, lane);
+        kst(kb, t * BN, len, lds + buf * 2 * TILE, wave);
+        vst(vb, t * BN, len, lds + buf * 2 * TILE + TILE, wave);
     };
     if (t0 < t1) stage(t0, 0);
     wait_loads();

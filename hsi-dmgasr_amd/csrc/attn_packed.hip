@@ -160,11 +160,12 @@ static Cut cut_queries(const hsidm_attn_desc* d, int es, int products) {
 }
 static Cut cut_keys(const hsidm_attn_desc* d, int es) {
     const int rb = row_bytes(d->D, es);
-    return cut_work(d, es, {rb <= 128 ? 2 : 1, d->D > 128 ? 6 : 4, true});
+    return cut_work(d, es, {rb <= 256 ? 2 : 1, d->D > 128 ? 6 : 4, true});
 }
 
+// (token strides: the kernels hold 64 rows' offsets in 32 bits)
 static bool rows_ok(const void* p, int64_t ts, int64_t hs, int es) {
-    return p && (uintptr_t)p % 16 == 0 && ts >= 0 && hs >= 0 && ts * es % 16 == 0 && hs * es % 16 == 0;
+    return p && (uintptr_t)p % 16 == 0 && ts >= 0 && hs >= 0 && ts <= (1 << 24) / es && ts * es % 16 == 0 && hs * es % 16 == 0;
 }
 static int check_attn(const hsidm_attn_desc* d, int& es) {
     if (!d || (d->prec != HSIDM_BF16 && d->prec != HSIDM_F16 && d->prec != HSIDM_F32X3)) return HSIDM_E_BADARG;

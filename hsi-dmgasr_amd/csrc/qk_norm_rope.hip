@@ -161,17 +161,24 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(RopeShape s, Rope
     reduce(dwk, out + s.D);
 }
 
-// dw[c] = sum over the workgroups' rows, in a fixed order, 64-bit sums; column c of part's 2 D
-__global__ __launch_bounds__(256) void rope_dw_kernel(const float* __restrict__ part, int rows, int D, float* __restrict__ dwq, float* __restrict__ dwk) {
-    __shared__ double red[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+// dw[c] = sum over the workgroups' rows, in a fixed order, 64-bit sums; column c of part's 2 D.  32 columns and 32 threads down the rows
+// per workgroup, four loads in flight each: the sums are latency, and with 4 threads down the rows this launch was a
+// third of a training pass (19215 tokens, 4 + 4 heads of 128: 101 -> 67 us).
+__global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__ part, int rows, int D, float* __restrict__ dwq, float* __restrict__ dwk) {
+    __shared__ double red[32][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
     double v = 0.0;
-    if (c < 2 * D)
-        for (int r = w; r < rows; r += 4) v += (double)part[(int64_t)r * 2 * D + c];
-    red[w][threadIdx.x & 63] = v;
+    const float* col = part + c;                                     // (2 D is a multiple of 32)
+    int r = y;
+    for (; r + 96 < rows; r += 128) {
+        const float a0 = col[(int64_t)r * 2 * D], a1 = col[(int64_t)(r + 32) * 2 * D], a2 = col[(int64_t)(r + 64) * 2 * D], a3 = col[(int64_t)(r + 96) * 2 * D];
+        v += (double)a0; v += (double)a1; v += (double)a2; v += (double)a3;
+    }
+    for (; r < rows; r += 32) v += (double)col[(int64_t)r * 2 * D];
+    red[y][x] = v;
     __syncthreads();
-    if (w == 0 && c < 2 * D) {
-        v = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    if (y == 0) {
+        for (int k = 1; k < 32; ++k) v += red[k][x];
         if (c < D) dwq[c] = (float)v; else dwk[c - D] = (float)v;
     }
 }
@@ -211,7 +218,7 @@ static void split_heads(RopeShape& s, int64_t token_blocks) {
     if (parts > 1) s.heads_per = (int)((heads + parts - 1) / parts);
 }
 
-constexpr int kBwdBlocks = 1024;             // four workgroups per CU, each with one row of dw sums
+constexpr int kBwdBlocks = 512;              // two workgroups per CU, each with one row of dw sums (1024: 67 instead of 64 us a training pass)
 
 static void bwd_grid(RopeShape& s, int& gx, int& gy) {
     const int64_t tb = (s.T * s.group + 255) / 256;
@@ -269,6 +276,6 @@ extern "C" int hsidm_qk_norm_rope_bwd(const hsidm_rope_desc* d, const void* d_ou
     else if (d->prec == HSIDM_F16) ROPE_BWD(f16);
     else ROPE_BWD(float);
 #undef ROPE_BWD
-    hipLaunchKernelGGL(rope_dw_kernel, dim3((2 * s.D + 63) / 64), dim3(256), 0, st, (const float*)workspace, gx * gy, s.D, dwq, dwk);
+    hipLaunchKernelGGL(rope_dw_kernel, dim3(2 * s.D / 32), dim3(1024), 0, st, (const float*)workspace, gx * gy, s.D, dwq, dwk);
     return (int)hipGetLastError();
 }

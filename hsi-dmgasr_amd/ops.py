@@ -573,9 +573,9 @@ def base(t):
 
 
 def rows_strided(t):
-    """Are the (token, head) rows of [T, H, D] contiguous along D and whole multiples of 16 bytes apart?"""
-    es = t.element_size()
-    return (t.stride(2) == 1 or t.shape[2] == 1) and all(t.shape[i] <= 1 or (t.stride(i) * es) % 16 == 0 and t.stride(i) > 0 for i in (0, 1))
+    """Are the (token, head) rows of [T, H, D] contiguous along D, whole multiples of 16 bytes apart, and tokens at most 16 MB?"""
+    es, (a, b, c), (n, h, d) = t.element_size(), t.stride(), t.shape
+    return (c == 1 or d == 1) and (n <= 1 or 0 < a * es <= 1 << 24 and a * es % 16 == 0) and (h <= 1 or b > 0 and b * es % 16 == 0)
 
 
 def rows_aligned(t):
@@ -590,7 +590,8 @@ def token_rows(t):
 
 def _strides(t):
     """(token, head) strides in elements; an axis of length one has whatever stride torch says: zero serves."""
-    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
+    (a, b, _), (n, h, _) = t.stride(), t.shape
+    return a if n > 1 else 0, b if h > 1 else 0
 
 
 class RotaryAxes:

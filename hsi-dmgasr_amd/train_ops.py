@@ -399,19 +399,23 @@ def attention_packed_bwd(do, q, k, v, out, saved, seqs, causal=False, scale=None
     the forward pass saved (its AttentionSaved).  grads: optional (dq, dk, dv) to write into, [T, H, D] views with 16-byte aligned rows
     (slices of a dqkv)."""
     d, _, nb, keep = ops.attn_desc(q, k, v, seqs, causal, scale)
-    T, Hq, _ = q.shape
+    shape, dtype, dev = q.shape, q.dtype, q.device
+    T, Hq, D = shape
     lse, lo = saved
-    for t in (do, out) + (() if lo is None else (lo,)):
-        if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
+    for t in (do, out, out if lo is None else lo):
+        if t.shape != shape or t.dtype != dtype or t.device != dev:
             raise ValueError("hsidm: do, out and its residual must be like q: %s %s, got %s %s" % (tuple(q.shape), q.dtype, tuple(t.shape), t.dtype))
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or lse.device != q.device:
+    if lse.dtype != torch.float32 or lse.shape != (Hq, T) or lse.device != dev:
         raise ValueError("hsidm: lse must be attention_packed's fp32 [%d, %d], got %s %s" % (Hq, T, lse.dtype, tuple(lse.shape)))
-    own = grads is None
-    if own:
-        grads = (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape))
-    for g, x in () if own else zip(grads, (q, k, v)):
-        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device or not ops.rows_aligned(g):
-            raise ValueError("hsidm: grads must be [T, H, D] tensors like q, k, v with 16-byte aligned rows")
+    if grads is None:
+        Hk = k.shape[1]
+        grads = (q.new_empty(shape), q.new_empty((T, Hk, D)), q.new_empty((T, Hk, D)))
+        strides = ((Hq * D, D), (Hk * D, D), (Hk * D, D))
+    else:
+        for g, x in zip(grads, (q, k, v)):
+            if g.shape != x.shape or g.dtype != dtype or g.device != dev or not ops.rows_aligned(g):
+                raise ValueError("hsidm: grads must be [T, H, D] tensors like q, k, v with 16-byte aligned rows")
+        strides = [ops._strides(g) for g in grads]
     dq, dk, dv = grads
     if T == 0:
         return dq, dk, dv
@@ -420,9 +424,9 @@ def attention_packed_bwd(do, q, k, v, out, saved, seqs, causal=False, scale=None
         ws = q.new_empty(nb, dtype=torch.uint8)
         do, out, lse = ops.token_rows(do), ops._aligned(out), lse.contiguous()
         lo = None if lo is None else ops._aligned(lo)
-        args = []
-        for t in (do, dq, dk, dv):
-            args += [t.data_ptr(), *ops._strides(t)]
+        args = [do.data_ptr(), *ops._strides(do)]
+        for t, st in zip(grads, strides):
+            args += [t.data_ptr(), *st]
         _check(L.hsidm_attention_packed_bwd(C.byref(d), out.data_ptr(), _lib.ptr(lo), lse.data_ptr(), *args, ws.data_ptr(), nb, _lib.stream_ptr()),
                "attention_packed_bwd")
     return dq, dk, dv

@@ -225,7 +225,7 @@ int hsidm_attention(int prec, const void* qkv, void* out, int B, int N, int C, v
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j]) v[j],   lse[h][i] = log sum_j exp(scale * q[i][h] . k[j])   (fp32 [Hq][T], may be
  *   NULL where no backward pass follows); scale > 0.
  * D <= 256 with rows of whole 16 bytes (multiples of 8, fp32: of 4); the last axis of q, k, v is contiguous, token and head strides (in
- * elements) are multiples of 16 bytes, bases 16-byte aligned; out [T][Hq][D] contiguous.  fp32 (exact fp32 products), bf16, fp16; scores,
+ * elements) are multiples of 16 bytes (tokens at most 16 MB apart), bases 16-byte aligned; out [T][Hq][D] contiguous.  fp32 (exact fp32 products), bf16, fp16; scores,
  * softmax and sums in fp32, probabilities rounded to the type ahead of their product with v.
  * Tiles (device memory, built by the caller once per set of lengths): for tile heights 64 and 128, the row ranges of every sequence of one
  * or more tokens - {first token of the sequence, its length, first row of the tile within it, 0} - n64 / n128 of them; qtiles: in the
