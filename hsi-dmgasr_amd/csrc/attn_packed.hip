@@ -170,7 +170,7 @@ static bool rows_ok(const void* p, int64_t ts, int64_t hs, int es) {
 static int check_attn(const hsidm_attn_desc* d, int& es) {
     if (!d || (d->prec != HSIDM_BF16 && d->prec != HSIDM_F16 && d->prec != HSIDM_F32X3)) return HSIDM_E_BADARG;
     es = d->prec == HSIDM_F32X3 ? 4 : 2;
-    if (d->T <= 0 || d->T > 0x7fffffff || d->Hk <= 0 || d->Hq <= 0 || d->Hq % d->Hk || d->Hq > 65535) return HSIDM_E_BADARG;
+    if (d->T <= 0 || d->T > 0x7fffff00 || d->Hk <= 0 || d->Hq <= 0 || d->Hq % d->Hk || d->Hq > 65535) return HSIDM_E_BADARG;
     if (d->D < 16 / es || d->D > 256 || d->D * es % 16) return HSIDM_E_BADARG;
     if (!(d->scale > 0.f) || !(d->scale < 1e30f)) return HSIDM_E_BADARG;
     if (!rows_ok(d->q, d->q_ts, d->q_hs, es) || !rows_ok(d->k, d->k_ts, d->k_hs, es) || !rows_ok(d->v, d->v_ts, d->v_hs, es)) return HSIDM_E_BADARG;

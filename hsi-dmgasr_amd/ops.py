@@ -695,8 +695,8 @@ class PackedSequences:
 
     def __init__(self, lengths, device="cuda"):
         self.lengths = tuple(int(n) for n in lengths)
-        if any(n < 0 for n in self.lengths) or sum(self.lengths) > 0x7fffffff:
-            raise ValueError("hsidm: sequence lengths must not be negative, nor more than 2^31 - 1 tokens together")
+        if any(n < 0 for n in self.lengths) or sum(self.lengths) > 0x7fffff00:
+            raise ValueError("hsidm: sequence lengths must not be negative, nor more than 2^31 - 256 tokens together")
         self.total, self.longest = sum(self.lengths), max(self.lengths, default=0)
         lens = np.asarray(self.lengths, dtype=np.int64)
         first = np.cumsum(lens) - lens
@@ -757,7 +757,8 @@ def _check_attn(q, k, v, seqs, causal, scale):
     nb = (0, 0)
     if T:
         d.q = d.k = d.v = d.qtiles64 & ~15                # (any aligned address: the sizes do not depend on it)
-        nb = (_lib.lib().hsidm_attention_packed_workspace_bytes(C.byref(d)), _lib.lib().hsidm_attention_packed_bwd_workspace_bytes(C.byref(d)))
+        with _lib.on_device(q.device):                    # (the split goes by the device's compute units)
+            nb = (_lib.lib().hsidm_attention_packed_workspace_bytes(C.byref(d)), _lib.lib().hsidm_attention_packed_bwd_workspace_bytes(C.byref(d)))
         if min(nb) < 0:
             _lib.check(int(min(nb)), "attention_packed_workspace_bytes")
     if in_place:

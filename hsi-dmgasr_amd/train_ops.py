@@ -2,6 +2,7 @@
 kernels enqueued on the current stream, nothing synchronised.  Forward convolutions and their input gradients go through
 ops.conv2d (the input gradient of a convolution is a convolution with the transposed, flipped weights)."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -344,9 +345,9 @@ def clip_coef(tensors, max_norm, grad_scale=1.0):
         raise ValueError("hsidm: max_norm and grad_scale must be positive, got %r and %r" % (max_norm, grad_scale))
     L, n, items = _lib.lib(), len(tl.tensors), tl.items()
     with _lib.on_device(tl.device):
-        ws = torch.empty(L.hsidm_grad_norm_workspace_bytes(n) // 8, dtype=torch.float64, device=tl.device)
-        out = torch.empty(2, dtype=torch.float32, device=tl.device)
-        _check(L.hsidm_grad_norm(items, n, float(grad_scale), float(max_norm), _lib.ptr(ws), _lib.ptr(out), _lib.stream_ptr()), "grad_norm")
+        new = tl.tensors[0].new_empty if n else functools.partial(torch.empty, device=tl.device)
+        ws, out = new(L.hsidm_grad_norm_workspace_bytes(n) // 8, dtype=torch.float64), new(2, dtype=torch.float32)
+        _check(L.hsidm_grad_norm(items, n, float(grad_scale), float(max_norm), ws.data_ptr(), out.data_ptr(), _lib.stream_ptr()), "grad_norm")
     return out
 
 
@@ -364,8 +365,9 @@ def clip_grad_norm_(tensors, max_norm):
     out = clip_coef(tl, max_norm)
     with _lib.on_device(tl.device):
         _check(_lib.lib().hsidm_scale_tensors(tl.items(), len(tl.tensors), _lib.ptr(out) + 4, _lib.stream_ptr()), "scale_tensors")
-    if tl.tensors:
-        torch.autograd.graph.increment_version(tl.tensors)      # written through raw pointers
+    written = [t for t in tl.tensors if not t.is_inference()]
+    if written:
+        torch.autograd.graph.increment_version(written)         # written through raw pointers
     return out[0]
 
 

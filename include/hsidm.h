@@ -220,7 +220,7 @@ int hsidm_film_affine(int prec, const void* x, const float* gamma_beta, void* ou
 int hsidm_attention(int prec, const void* qkv, void* out, int B, int N, int C, void* stream);
 
 /* ---- attention over packed sequences ------------------------------------------------------------------------------------------
- * T tokens of several sequences, one behind the other: q [T][Hq][D], k, v [T][Hk][D] (Hk divides Hq; query head h uses key head
+ * T tokens (at most 2^31 - 256) of several sequences, one behind the other: q [T][Hq][D], k, v [T][Hk][D] (Hk divides Hq; query head h uses key head
  * h / (Hq / Hk)); every token attends to the tokens of its own sequence - causal: to those up to itself.
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j]) v[j],   lse[h][i] = log sum_j exp(scale * q[i][h] . k[j])   (fp32 [Hq][T], may be
  *   NULL where no backward pass follows); scale > 0.

@@ -90,7 +90,7 @@ def test_sequences_and_their_tiles():
             work = {"full": got[:, 1], "causal q": [min(x[1], x[2] + rows) for x in got], "causal k": got[:, 1] - got[:, 2]}[kind]
             assert all(a >= b for a, b in zip(work, work[1:]))
     assert ops.PackedSequences([], device="cpu").total == 0 and ops.PackedSequences([0], device="cpu").n64 == 0
-    for bad in ([-1], [2 ** 31], [2 ** 30, 2 ** 30]):
+    for bad in ([-1], [2 ** 31], [2 ** 30, 2 ** 30], [2 ** 31 - 255]):
         with pytest.raises(ValueError):
             ops.PackedSequences(bad, device="cpu")
 
@@ -353,3 +353,33 @@ def test_captured_and_on_another_stream(dev, lengths):
         other = step()
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+@GPU
+def test_offsets_beyond_32_bits(dev):
+    """More than 2^31 elements of queries, keys in rows 128 KB apart and 18 MB apart (through a copy): the last sequence is what it is alone."""
+    from hsi_dmgasr_amd import ops
+    from hsi_dmgasr_amd import train_ops as Tr
+    n, H, D = 8, 512, 128
+    T = 33000
+    lengths = [n] * (T // n)
+    q = torch.randn(T, H, D, device=dev, dtype=torch.bfloat16)
+    assert q.numel() > 2 ** 31
+    k, v = q[:, 5:6], q[:, 300:301]
+    seqs, one = ops.PackedSequences(lengths, device=dev), ops.PackedSequences([n], device=dev)
+    o, saved = ops.attention_packed(q, k, v, seqs, causal=True, want_lse=True)
+    last = [t[-n:].clone() for t in (q, k, v)]
+    o1, saved1 = ops.attention_packed(*last, one, causal=True, want_lse=True)
+    assert torch.equal(o[-n:], o1) and torch.equal(saved.lse[:, -n:], saved1.lse)
+    g = Tr.attention_packed_bwd(q, q, k, v, o, saved, seqs, causal=True)
+    g1 = Tr.attention_packed_bwd(last[0], *last, o1, saved1, one, causal=True)
+    assert torch.equal(g[0][-n:], g1[0])
+    # dk and dv add 512 heads in fp32, split between workgroups or not: sums of the same terms in another order, then one rounding
+    for a, b in zip(g[1:], g1[1:]):
+        assert float((a[-n:].double() - b.double()).abs().max()) <= 2 * 2.0 ** -8 * float(b.double().abs().max())
+    del o, saved, g
+    far = torch.randn(100 * 70000, 128, device=dev, dtype=torch.bfloat16).view(100, 70000, 128)      # 17.9 MB from token to token
+    qf = far[:, 1:3]
+    s100 = ops.PackedSequences([100], device=dev)
+    assert not ops.rows_strided(qf)
+    assert torch.equal(ops.attention_packed(qf, qf, qf, s100), ops.attention_packed(qf.clone(), qf.clone(), qf.clone(), s100))

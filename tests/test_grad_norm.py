@@ -290,3 +290,25 @@ def test_trainer_with_clipping_on_the_device(dev):
         # (a captured step reads its bias corrections as two fp32 words: one rounding more)
         assert float((p - tr.flat).abs().max()) <= 1e-3 * 1e-5 + 2.0 ** -23 * float(p.abs().max())
         assert torch.equal(m, tr.m) and torch.equal(v, tr.v)
+
+
+@GPU
+def test_more_than_32_bits_of_elements(dev):
+    """One tensor of 2^31 + 5 elements among small ones, to the last element (its value and half of it are powers of two)."""
+    from hsi_dmgasr_amd import train_ops as T
+    n = 2 ** 31 + 5
+    big = torch.full((n,), 2.0 ** -15, device=dev, dtype=torch.bfloat16)
+    small = torch.zeros(3, device=dev)
+    want = 2.0 ** -15 * math.sqrt(n)
+    assert abs(float(T.grad_norm([small, big])) - want) <= (half_step(torch.float32) + 1e-12) * want
+    T.clip_grad_norm_([small, big], want / 2 + 1e-6)                # (the coefficient is within 1e-5 of a half; bf16 keeps eight bits)
+    assert float(big[-1]) == 2.0 ** -16 and float(big[0]) == 2.0 ** -16 and float(big[2 ** 30]) == 2.0 ** -16
+
+
+@GPU
+def test_clip_of_inference_tensors(dev):
+    from hsi_dmgasr_amd import train_ops as T
+    with torch.inference_mode():
+        x = torch.full((4,), 3.0, device=dev)
+        assert float(T.clip_grad_norm_([x], 3.0)) == 6.0
+        assert abs(float(x[0]) - 1.5) < 1e-6

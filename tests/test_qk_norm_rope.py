@@ -239,3 +239,21 @@ def test_captured_and_on_another_stream(dev):
         other = step()
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+@GPU
+def test_offsets_beyond_32_bits(dev):
+    from hsi_dmgasr_amd import ops
+    from hsi_dmgasr_amd import train_ops as Tr
+    T, H, D = 33000, 512, 128
+    q = torch.randn(T, H, D, device=dev, dtype=torch.bfloat16)
+    k = q[:, 7:9]
+    w = torch.rand(D, device=dev) + 0.5
+    pos = torch.randint(0, 500, (T, 2), device=dev, dtype=torch.int32)
+    axes = ops.RotaryAxes((32, 32), D, device=dev)
+    oq, ok = ops.qk_norm_rope(q, k, w, w, pos, axes)
+    lq, lk = ops.qk_norm_rope(q[-5:].clone(), k[-5:].clone(), w, w, pos[-5:].contiguous(), axes)
+    assert torch.equal(oq[-5:], lq) and torch.equal(ok[-5:], lk)
+    g = Tr.qk_norm_rope_bwd(oq, ok, q, k, w, w, pos, axes)
+    g1 = Tr.qk_norm_rope_bwd(lq, lk, q[-5:].clone(), k[-5:].clone(), w, w, pos[-5:].contiguous(), axes)
+    assert torch.equal(g[0][-5:], g1[0]) and torch.equal(g[1][-5:], g1[1])
