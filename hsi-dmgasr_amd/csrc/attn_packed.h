@@ -216,9 +216,9 @@ __device__ __forceinline__ void store_residual(T* out, const f32x16& acc, float 
 
 // Workgroup -> (tile, head): all heads of a tile follow each other (the tiles come heaviest first, and a late heavy one would leave
 // the chip waiting), heads that share keys on one XCD (workgroups go to the eight XCDs in turn, each with an L2 of its own).
-__device__ __forceinline__ void which_tile(int heads, int& tile, int& head) {
-    tile = blockIdx.x / heads;
-    const int j = blockIdx.x - tile * heads;
+__device__ __forceinline__ void which_tile(int block, int heads, int& tile, int& head) {
+    tile = block / heads;
+    const int j = block - tile * heads;
     head = (heads & 7) == 0 ? (j & 7) * (heads >> 3) + (j >> 3) : j;
 }
 
@@ -239,16 +239,16 @@ struct AttnFwdArgs {
 // are fp32 in any case).  NW waves of 32 queries each walk the key tiles together; two LDS buffers: a tile arrives while the one
 // before it is multiplied.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_fwd_kernel(AttnFwdArgs a) {
+__global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 512 ? 2 : 1)) void attn_fwd_kernel(AttnFwdArgs a) {
     typedef Row<T, DP> R;
     constexpr int BN = R::BYTES <= 256 ? 64 : 32, ND = DP / 32, TILE = BN * R::BYTES;
     // Where the accumulators spill over into the second half of the register file, a jump around work on them costs a move of every one of
     // them on either way: such kernels do masked tiles too and rescale every time.
-    constexpr bool SKIP = R::BYTES <= 256;
+    constexpr bool SKIP = R::BYTES <= 512;
     extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, h = lane >> 5;
     int ti, head;
-    which_tile(a.Hq, ti, head);
+    which_tile(blockIdx.x, a.Hq, ti, head);
     const AttnTile tile = a.tiles[ti];
     const int len = tile.len, q0 = tile.row0 + wave * 32, kvh = head / (a.Hq / a.Hk), pieces = a.D * (int)sizeof(T) / 16;
     const char* kb = a.k.p + (int64_t)tile.start * a.k.ts + kvh * a.k.hs;
@@ -391,24 +391,24 @@ template <typename T> __device__ __forceinline__ void store_grad(const AttnTenso
 template <typename T, int DP> struct KvTiles { static constexpr int ND = DP > 128 ? DP / 64 : DP / 32, PARTS = DP / 32 / ND; };
 
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_bwd_kv_kernel(AttnBwdArgs a) {
+__device__ __forceinline__ void attn_bwd_kv(const AttnBwdArgs& a, char* lds, int block, int share, int part) {
     typedef Row<T, DP> R;
     constexpr int BQ = R::BYTES <= 256 ? 64 : 32, ND = KvTiles<T, DP>::ND, TILE = BQ * R::BYTES, BUF = 2 * TILE + 512;
-    extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][Q tile, dO tile, lse[64], delta[64]]
+    // lds: [2][Q tile, dO tile, lse[64], delta[64]]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, h = lane >> 5;
     int ti, kvh;
-    which_tile(a.Hk, ti, kvh);
+    which_tile(block, a.Hk, ti, kvh);
     const AttnTile tile = a.tiles[ti];
     const int len = tile.len, k0 = tile.row0 + wave * 32, group = a.Hq / a.Hk, pieces = a.D * (int)sizeof(T) / 16;
     // this workgroup's work: the query tiles that see its keys, for every head of the group, one head behind the other
     const int tq0 = a.causal ? tile.row0 / BQ : 0, ntq = (len + BQ - 1) / BQ - tq0, work = ntq * group;
-    const int per = (work + a.splits - 1) / a.splits, w0 = blockIdx.y * per, w1 = min(work, w0 + per);
+    const int per = (work + a.splits - 1) / a.splits, w0 = share * per, w1 = min(work, w0 + per);
     const int key = k0 + lr, keyc = min(key, len - 1);
     u32x4 kf[R::STEPS], vf[R::STEPS];
     load_row<T, DP>(a.k.p + (int64_t)(tile.start + keyc) * a.k.ts + kvh * a.k.hs, pieces, h, kf);
     load_row<T, DP>(a.v.p + (int64_t)(tile.start + keyc) * a.v.ts + kvh * a.v.hs, pieces, h, vf);
     const Places<T, DP> at(lane);
-    const int dbytes = blockIdx.z * ND * 32 * (int)sizeof(T);        // this workgroup's part of D
+    const int dbytes = part * ND * 32 * (int)sizeof(T);        // this workgroup's part of D
     f32x16 dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) { zero16(dk[d]); zero16(dv[d]); }
@@ -483,17 +483,17 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
     const int64_t token = (int64_t)tile.start + key;
     const float fk = a.scale * GradScale<T>::p_back / f, fv = GradScale<T>::p_back;
     if (a.splits > 1) {
-        float* out = a.part + (((int64_t)blockIdx.y * 2 * a.T + token) * a.Hk + kvh) * a.D;
+        float* out = a.part + (((int64_t)share * 2 * a.T + token) * a.Hk + kvh) * a.D;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const int d0 = 32 * (blockIdx.z * ND + d);
+            const int d0 = 32 * (part * ND + d);
             store_column<float>(out, dk[d], fk, d0, h, a.D);
             store_column<float>(out + a.T * a.Hk * a.D, dv[d], fv, d0, h, a.D);
         }
     } else {
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const int d0 = 32 * (blockIdx.z * ND + d);
+            const int d0 = 32 * (part * ND + d);
             store_grad<T>(a.dk, token, kvh, dk[d], fk, d0, h, a.D);
             store_grad<T>(a.dv, token, kvh, dv[d], fv, d0, h, a.D);
         }
@@ -502,21 +502,21 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
 
 // dQ of 32 queries per wave
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_bwd_q_kernel(AttnBwdArgs a) {
+__device__ __forceinline__ void attn_bwd_q(const AttnBwdArgs& a, char* lds, int block, int share) {
     typedef Row<T, DP> R;
     constexpr int BN = R::BYTES <= 256 ? 64 : 32, ND = DP / 32, TILE = BN * R::BYTES;
     constexpr bool SKIP = R::BYTES <= 256;                           // (as in the forward kernel)
-    extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K tile, V tile]
+    // lds: [2][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, h = lane >> 5;
     int ti, head;
-    which_tile(a.Hq, ti, head);
+    which_tile(block, a.Hq, ti, head);
     const AttnTile tile = a.tiles[ti];
     const int len = tile.len, q0 = tile.row0 + wave * 32, kvh = head / (a.Hq / a.Hk), pieces = a.D * (int)sizeof(T) / 16;
     const char* kb = a.k.p + (int64_t)tile.start * a.k.ts + kvh * a.k.hs;
     const char* vb = a.v.p + (int64_t)tile.start * a.v.ts + kvh * a.v.hs;
     const int kend = a.causal ? min(len, tile.row0 + 32 * NW) : len;
     const int nkt = (kend + BN - 1) / BN, per = (nkt + a.splits - 1) / a.splits;
-    const int t0 = blockIdx.y * per, t1 = min(nkt, t0 + per);
+    const int t0 = share * per, t1 = min(nkt, t0 + per);
     const int row = q0 + lr, rowc = min(row, len - 1);
     const int64_t rtok = (int64_t)tile.start + rowc;
     u32x4 qf[R::STEPS], gf[R::STEPS];
@@ -575,7 +575,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
     if (row >= len) return;
     const float fq = a.scale * GradScale<T>::p_back / f;
     if (a.splits > 1) {
-        float* out = a.part + (((int64_t)blockIdx.y * a.T + rtok) * a.Hq + head) * a.D;
+        float* out = a.part + (((int64_t)share * a.T + rtok) * a.Hq + head) * a.D;
 #pragma unroll
         for (int d = 0; d < ND; ++d) store_column<float>(out, dq[d], fq, 32 * d, h, a.D);
     } else {
@@ -584,9 +584,26 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
     }
 }
 
+// Both in one launch, the key tiles' workgroups first: neither depends on the other, and the query tiles fill what the key tiles leave
+// free - a launch of its own would begin when the last of them ends (fp16 4 x 256 x 8 heads of 64: 25 us one after the other, DESIGN's table).
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_bwd_kernel(AttnBwdArgs kv, AttnBwdArgs q, int kv_blocks, int q_blocks) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    int b = blockIdx.x;
+    const int kv_all = kv_blocks * kv.splits * KvTiles<T, DP>::PARTS;
+    if (b < kv_all) {
+        const int rest = b / kv_blocks;
+        attn_bwd_kv<T, DP, NW>(kv, lds, b - rest * kv_blocks, rest % kv.splits, rest / kv.splits);
+    } else {
+        b -= kv_all;
+        attn_bwd_q<T, DP, NW>(q, lds, b % q_blocks, b / q_blocks);
+    }
+}
+
 // ---- launches: one translation unit per element type (attn_packed_<type>.hip) ---------------------------------------------------
 // kind: which kernel; waves: 2 or 4 per workgroup (a tile is 32 rows per wave)
-enum { ATTN_FWD = 0, ATTN_BWD_KV = 1, ATTN_BWD_Q = 2 };
+enum { ATTN_FWD = 0, ATTN_BWD = 1 };
+struct AttnBwdPair { AttnBwdArgs kv, q; int kv_tiles, q_tiles; };
 template <typename T> int attn_launch(int kind, const void* args, int waves, int ntiles, hipStream_t s);
 extern template int attn_launch<bf16>(int, const void*, int, int, hipStream_t);
 extern template int attn_launch<f16>(int, const void*, int, int, hipStream_t);

@@ -39,17 +39,21 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
     }
 }
 
-// out[t][h][d] = sum over the shares of part[s * share + (t * H + h) * D + d], in order
+// out[t][h][d] = sum over the shares of part[s * share + (t * H + h) * D + d], in order; up to three such sums (dK, dV, dQ) in one launch
+struct AttnSum { const float* part; int64_t share; AttnTensor out; int S, H; };
+struct AttnSums { AttnSum s[3]; };
+
 template <typename T>
-__global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__ part, int S, int64_t share, int64_t T_, int H, int D, AttnTensor out) {
+__global__ __launch_bounds__(256) void attn_add_kernel(AttnSums sums, int64_t T_, int D) {
+    const AttnSum a = sums.s[blockIdx.y];
     const int per_row = D / 4;
-    const int64_t n = T_ * H * per_row;
+    const int64_t n = T_ * a.H * per_row;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / per_row, token = row / H;
-        const int d = (int)(i - row * per_row) * 4, head = (int)(row - token * H);
+        const int64_t row = i / per_row, token = row / a.H;
+        const int d = (int)(i - row * per_row) * 4, head = (int)(row - token * a.H);
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < S; ++s) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(part + s * share + row * D + d);
+        for (int s = 0; s < a.S; ++s) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + s * a.share + row * D + d);
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] += x[k];
         }
@@ -57,7 +61,7 @@ __global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__
         vec r;
 #pragma unroll
         for (int k = 0; k < 4; ++k) r[k] = (T)v[k];
-        *reinterpret_cast<vec*>(reinterpret_cast<T*>(const_cast<char*>(out.p) + token * out.ts + head * out.hs) + d) = r;
+        *reinterpret_cast<vec*>(reinterpret_cast<T*>(const_cast<char*>(a.out.p) + token * a.out.ts + head * a.out.hs) + d) = r;
     }
 }
 
@@ -131,12 +135,13 @@ static int tile_rows(int D, int es) { return row_bytes(D, es) <= 256 ? 64 : 32; 
 //   plus the shares' partial sums, written in fp32 and read again.
 // The rates are what the kernels reach (a step of the measured cases comes out within 15 %); shares stay at four steps or more.
 struct Walk { int resident, products; bool kv; };            // workgroups of four waves per CU (by registers), matrix products per tile pair
-static Cut cut_work(const hsidm_attn_desc* d, int es, const Walk& k) {
+// waves: 0 to choose, 2 or 4 to go with another kernel's tiles
+static Cut cut_work(const hsidm_attn_desc* d, int es, const Walk& k, int waves) {
     const int heads = k.kv ? d->Hk : d->Hq, walks = k.kv ? d->Hq / d->Hk : 1, rows = tile_rows(d->D, es), width = row_bytes(d->D, es) / es;
     const int64_t steps = (d->longest + rows - 1) / rows * walks;
     const double cus = device_cus(), rate = es == 4 ? 105e12 : width <= 32 ? 250e12 : width <= 64 ? 600e12 : 750e12;
     Cut c;
-    c.waves = (double)d->n128 * heads >= 0.5 * cus || steps >= 16 ? 4 : 2;
+    c.waves = waves ? waves : (double)d->n128 * heads >= 0.5 * cus || steps >= 16 ? 4 : 2;
     c.ntiles = c.waves == 4 ? d->n128 : d->n64;
     const int tile = 32 * c.waves;
     const double slots = cus * k.resident * (4 / c.waves), n = (double)c.ntiles * heads;
@@ -154,13 +159,13 @@ static Cut cut_work(const hsidm_attn_desc* d, int es, const Walk& k) {
     }
     return c;
 }
-static Cut cut_queries(const hsidm_attn_desc* d, int es, int products) {
+static Cut cut_queries(const hsidm_attn_desc* d, int es, int products, int waves = 0) {
     const int rb = row_bytes(d->D, es);
-    return cut_work(d, es, {rb <= 128 ? 3 : rb <= 256 ? 2 : 1, products, false});
+    return cut_work(d, es, {rb <= 128 ? 3 : rb <= (products == 2 ? 512 : 256) ? 2 : 1, products, false}, waves);
 }
 static Cut cut_keys(const hsidm_attn_desc* d, int es) {
     const int rb = row_bytes(d->D, es);
-    return cut_work(d, es, {rb <= 256 ? 2 : 1, d->D > 128 ? 6 : 4, true});
+    return cut_work(d, es, {rb <= 256 ? 2 : 1, d->D > 128 ? 6 : 4, true}, 0);
 }
 
 // (token strides: the kernels hold 64 rows' offsets in 32 bits)
@@ -187,21 +192,20 @@ static int launch(int prec, int kind, const void* args, const Cut& c, hipStream_
 }
 static unsigned blocks_for(int64_t n) { const int64_t b = (n + 255) / 256; return (unsigned)(b < 65536 ? b : 65536); }
 
-struct BwdPlan { Cut q, kv; int64_t delta, maxima, part, bytes; int nmax; };
+struct BwdPlan { Cut q, kv; int64_t delta, maxima, part_kv, part_q, bytes; int nmax; };
 static BwdPlan bwd_plan(const hsidm_attn_desc* d, int es) {
     BwdPlan p;
-    p.q = cut_queries(d, es, 3);
     p.kv = cut_keys(d, es);
+    p.q = cut_queries(d, es, 3, p.kv.waves);                          // (one launch: one tile height)
     int group = 1;
     while (group < d->D * es / 16) group *= 2;
     const int64_t rows = d->T * d->Hq, blocks = (rows * group + 255) / 256;
     p.nmax = (int)(blocks < kDeltaBlocks ? blocks : kDeltaBlocks);
     p.delta = 0;
     p.maxima = up16(rows * 4);
-    p.part = p.maxima + up16((int64_t)p.nmax * 8);
-    const int64_t pq = p.q.splits > 1 ? (int64_t)p.q.splits * d->T * d->Hq * d->D * 4 : 0;
-    const int64_t pkv = p.kv.splits > 1 ? (int64_t)p.kv.splits * 2 * d->T * d->Hk * d->D * 4 : 0;
-    p.bytes = p.part + (pq > pkv ? pq : pkv);                         // (one after the other on the stream: they share the space)
+    p.part_kv = p.maxima + up16((int64_t)p.nmax * 8);
+    p.part_q = p.part_kv + (p.kv.splits > 1 ? (int64_t)p.kv.splits * 2 * d->T * d->Hk * d->D * 4 : 0);
+    p.bytes = p.part_q + (p.q.splits > 1 ? (int64_t)p.q.splits * d->T * d->Hq * d->D * 4 : 0);
     return p;
 }
 
@@ -213,13 +217,8 @@ static void launch_delta(const AttnTensor& dout, const AttnTensor& o, const void
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_delta_kernel<T>), dim3(nmax), dim3(256), 0, s, dout, o, (const char*)lo, v, d->T, d->Hq, d->Hk, pieces, group, delta, maxima);
 }
 template <typename T>
-static void launch_add(const float* part, const Cut& c, int64_t share, int64_t T_, int H, int D, const AttnTensor& out, hipStream_t s) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_add_kernel<T>), dim3(blocks_for(T_ * H * D / 4)), dim3(256), 0, s, part, c.splits, share, T_, H, D, out);
-}
-static void add_parts(int prec, const float* part, const Cut& c, int64_t share, int64_t T_, int H, int D, const AttnTensor& out, hipStream_t s) {
-    if (prec == HSIDM_BF16) launch_add<bf16>(part, c, share, T_, H, D, out, s);
-    else if (prec == HSIDM_F16) launch_add<f16>(part, c, share, T_, H, D, out, s);
-    else launch_add<float>(part, c, share, T_, H, D, out, s);
+static void launch_add(const AttnSums& sums, int n, int heads, int64_t T_, int D, hipStream_t s) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_add_kernel<T>), dim3(blocks_for(T_ * heads * D / 4), n), dim3(256), 0, s, sums, T_, D);
 }
 
 }  // namespace hsidm
@@ -285,24 +284,36 @@ extern "C" int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* 
     a.q = tensor(d->q, d->q_ts, d->q_hs, es); a.k = tensor(d->k, d->k_ts, d->k_hs, es); a.v = tensor(d->v, d->v_ts, d->v_hs, es);
     a.dout = tensor(dout, do_ts, do_hs, es);
     a.dq = tensor(dq, dq_ts, dq_hs, es); a.dk = tensor(dk, dk_ts, dk_hs, es); a.dv = tensor(dv, dv_ts, dv_hs, es);
-    a.lse = lse; a.delta = delta; a.maxima = maxima; a.part = (float*)(ws + p.part);
+    a.lse = lse; a.delta = delta; a.maxima = maxima;
     a.T = d->T; a.Hq = d->Hq; a.Hk = d->Hk; a.D = d->D; a.causal = d->causal; a.nmax = p.nmax; a.scale = d->scale;
     const AttnTensor o = tensor(out, (int64_t)d->Hq * d->D, d->D, es);
     const int pieces = d->D * es / 16;
     if (d->prec == HSIDM_BF16) launch_delta<bf16>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
     else if (d->prec == HSIDM_F16) launch_delta<f16>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
     else launch_delta<float>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
-    a.splits = p.kv.splits;
-    a.tiles = (const AttnTile*)(p.kv.waves == 4 ? d->ktiles128 : d->ktiles64);
-    if (int rc = launch(d->prec, ATTN_BWD_KV, &a, p.kv, s)) return rc;
-    if (a.splits > 1) {
+    const bool tall = p.kv.waves == 4;
+    AttnBwdPair pair = {a, a, p.kv.ntiles, p.q.ntiles};
+    pair.kv.splits = p.kv.splits; pair.kv.part = (float*)(ws + p.part_kv);
+    pair.kv.tiles = (const AttnTile*)(tall ? d->ktiles128 : d->ktiles64);
+    pair.q.splits = p.q.splits; pair.q.part = (float*)(ws + p.part_q);
+    pair.q.tiles = (const AttnTile*)(tall ? d->qtiles128 : d->qtiles64);
+    if (int rc = launch(d->prec, ATTN_BWD, &pair, p.kv, s)) return rc;
+    AttnSums sums;
+    int n = 0, heads = 0;
+    if (p.kv.splits > 1) {
         const int64_t one = d->T * d->Hk * d->D;
-        add_parts(d->prec, a.part, p.kv, 2 * one, d->T, d->Hk, d->D, a.dk, s);
-        add_parts(d->prec, a.part + one, p.kv, 2 * one, d->T, d->Hk, d->D, a.dv, s);
+        sums.s[n++] = {pair.kv.part, 2 * one, a.dk, p.kv.splits, d->Hk};
+        sums.s[n++] = {pair.kv.part + one, 2 * one, a.dv, p.kv.splits, d->Hk};
+        heads = d->Hk;
     }
-    a.splits = p.q.splits;
-    a.tiles = (const AttnTile*)(p.q.waves == 4 ? d->qtiles128 : d->qtiles64);
-    if (int rc = launch(d->prec, ATTN_BWD_Q, &a, p.q, s)) return rc;
-    if (a.splits > 1) add_parts(d->prec, a.part, p.q, d->T * d->Hq * d->D, d->T, d->Hq, d->D, a.dq, s);
+    if (p.q.splits > 1) {
+        sums.s[n++] = {pair.q.part, d->T * d->Hq * d->D, a.dq, p.q.splits, d->Hq};
+        heads = d->Hq;
+    }
+    if (n) {
+        if (d->prec == HSIDM_BF16) launch_add<bf16>(sums, n, heads, d->T, d->D, s);
+        else if (d->prec == HSIDM_F16) launch_add<f16>(sums, n, heads, d->T, d->D, s);
+        else launch_add<float>(sums, n, heads, d->T, d->D, s);
+    }
     return (int)hipGetLastError();
 }
