@@ -238,12 +238,15 @@ struct AttnFwdArgs {
 // follows the true one lazily: only when some query's grew by more than 2^8 are they rescaled (fp16 probabilities stay below 2^8, sums
 // are fp32 in any case).  NW waves of 32 queries each walk the key tiles together; two LDS buffers: a tile arrives while the one
 // before it is multiplied.
+// Bound by the matrix pipe and the exponentials beside it (at D = 64 the vector unit has 680 cycles of work per 512 of the matrix pipe's).
+// fp16, 2 x 16384 tokens, one head of 64: 188 us, 730 TFLOP/s; bf16 causal, 20115 tokens in six sequences, 16 / 4 heads of 128: 515 us, 905
+// TFLOP/s of the pairs that count; fp32 (exact products, peak 157), 2 x 4096 tokens of 128: 151 us, 114 TFLOP/s.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 512 ? 2 : 1)) void attn_fwd_kernel(AttnFwdArgs a) {
     typedef Row<T, DP> R;
     constexpr int BN = R::BYTES <= 256 ? 64 : 32, ND = DP / 32, TILE = BN * R::BYTES;
-    // Where the accumulators spill over into the second half of the register file, a jump around work on them costs a move of every one of
-    // them on either way: such kernels do masked tiles too and rescale every time.
+    // Where the accumulators reach into the second half of the register file (fp32, D > 128), a jump around work on them costs a move of every
+    // one of them on either way: that kernel does masked tiles too and rescales every time.
     constexpr bool SKIP = R::BYTES <= 512;
     extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, h = lane >> 5;
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 512 ? 2 : 1)) void a
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------
 //   P = exp(S - lse), dP = dO V^T, delta = rowsum(dO o O), dS = P o (dP - delta):  dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO
-// Two kernels recompute S and dP: one owns key tiles and walks the queries of every head that shares them (dK, dV: the sum over a group's
+// Two kinds of workgroups recompute S and dP: one owns key tiles and walks the queries of every head that shares them (dK, dV: the sum over a group's
 // heads stays in registers), one owns query tiles and walks the keys (dQ).  Nothing is added atomically: results do not depend on order.
 // fp16: P and dS are stored to 11 bits with exponents down to 2^-14 only, and both shrink with the number of keys and the gradient's
 // size.  P is kept times 2^10 and dS times a power of two chosen from max |dO| and max |V| (|dP - delta| <= 2 |dO| |V|): neither
@@ -585,7 +588,11 @@ __device__ __forceinline__ void attn_bwd_q(const AttnBwdArgs& a, char* lds, int 
 }
 
 // Both in one launch, the key tiles' workgroups first: neither depends on the other, and the query tiles fill what the key tiles leave
-// free - a launch of its own would begin when the last of them ends (fp16 4 x 256 x 8 heads of 64: 25 us one after the other, DESIGN's table).
+// free - a launch of its own would begin when the last of them ends (fp16 4 x 256 tokens, 8 heads of 64: 13 us instead of 25; bf16 causal,
+// 10739 tokens in five sequences, 8 / 2 heads of 128: 304 us instead of 412).
+// Bound by the matrix pipe together with the vector work and the LDS reads between its instructions (four products per pair of tiles read
+// 32 KB a wave at D = 128, as long as they multiply).  8 x 2048 tokens, 16 heads, bf16: D = 128 1095 us, D = 64 529 us - 880 and 910
+// TFLOP/s of the seven products that run (two of them recompute S and dP); fp32, 2 x 4096 tokens of 128: 528 us, 114 TFLOP/s.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_bwd_kernel(AttnBwdArgs kv, AttnBwdArgs q, int kv_blocks, int q_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];

@@ -5,6 +5,9 @@
 // A lane holds 8 elements of the first half of a head and the 8 they pair with, so the rotation needs no exchange; D/16 lanes (rounded up
 // to a power of two) share a head, and walk the token's heads with ONE set of sines and cosines: those are the costly part - the angle is
 // formed in 64 bits, as turns, and only its fraction is rounded, so that far positions (10^5 and more radians) keep their angle.
+// 5 x 128 x 128 tokens, 8 + 2 heads of 64, bf16: 50 us, 4.2 TB/s (a large copy reaches 4.9); 19215 tokens, 4 + 4 heads of 128, fp16: forward 17
+// us, backward 37 + 4 us.  Tried and not kept: stores past the caches (backward 9 % faster, forward 11 % slower, and the next kernel reads the
+// result), more than one workgroup per token block once every CU has two.
 #include "common.h"
 #include "../../include/hsidm.h"
 
