@@ -612,6 +612,9 @@ class RotaryAxes:
         self.freq = torch.tensor(turns or [0.0], dtype=torch.float64).to(device)
         self._plans = {}                                  # (rope_desc)
 
+    def __getstate__(self):                               # (the plans point at this object's table)
+        return {**self.__dict__, "_plans": {}}
+
 
 def _check_rope(q, k, wq, wk, pos, axes, eps):
     """Everything about a call but its addresses: (descriptor without them, backward workspace bytes, whether all tensors are read in place)."""
@@ -717,6 +720,9 @@ class PackedSequences:
         self.device = self._tables.device
         self._plans = {}                                  # (attn_desc)
 
+    def __getstate__(self):                               # copies and pickles of a module that holds one: the plans point at this object's tables
+        return {**self.__dict__, "_plans": {}}
+
     def pairs(self, causal):
         """(query, key) pairs of one head."""
         return sum(n * (n + 1) // 2 if causal else n * n for n in self.lengths)
@@ -794,7 +800,7 @@ def attention_packed(q, k, v, seqs, causal=False, scale=None, want_lse=False):
     """softmax(scale * q k^T) v within every sequence of a packed batch: q [T, Hq, D], k / v [T, Hk, D] (Hk divides Hq; any strides, rows
     on 16-byte boundaries are read in place), seqs a PackedSequences over the T tokens; causal: a token sees itself and what came
     before; scale: 1/sqrt(D) unless given.  Any length - nothing of size length^2 is stored.  -> out [T, Hq, D] in q's type, with
-    want_lse also the AttentionSaved that train_ops.attention_packed_bwd takes."""
+    want_lse also the AttentionSaved that train_ops.attention_packed_bwd takes (autograd does not record the call)."""
     d, nb, _, keep = attn_desc(q, k, v, seqs, causal, scale)
     out = q.new_empty(q.shape)
     lse = lo = None

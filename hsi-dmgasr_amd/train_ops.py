@@ -357,9 +357,12 @@ def grad_norm(tensors, grad_scale=1.0):
 
 
 def clip_grad_norm_(tensors, max_norm):
-    """Scales the tensors in place so that their global 2-norm is at most max_norm; returns the norm from before as a 0-dim fp32 device
-    tensor (torch.nn.utils.clip_grad_norm_ over gradients).  The tensors must not overlap (a shared one would be scaled twice)."""
+    """Scales the tensors - the GRADIENTS themselves, not the parameters - in place so that their global 2-norm is at most max_norm; returns
+    the norm from before as a 0-dim fp32 device tensor (torch.nn.utils.clip_grad_norm_'s definition).  The tensors must not overlap (a
+    shared one would be scaled twice)."""
     tl = tensors if isinstance(tensors, TensorList) else TensorList(tensors)
+    if any(t.requires_grad for t in tl.tensors):
+        raise ValueError("hsidm: clip_grad_norm_ scales the tensors it is given: pass [p.grad for p in parameters], not the parameters")
     if not tl.disjoint():
         raise ValueError("hsidm: clip_grad_norm_ needs tensors that do not overlap (is one of them listed twice?)")
     out = clip_coef(tl, max_norm)

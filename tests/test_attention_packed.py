@@ -138,12 +138,33 @@ def test_refusals_without_a_gpu():
     assert L.hsidm_attention_packed_bwd(desc(), one, None, one, *[one, 256, 63] * 4, one, need, None) == -1
 
 
+def test_structs_match_the_header(tmp_path):
+    """Sizes and offsets of the descriptors that the ctypes binding restates, as the C compiler lays them out."""
+    import os
+    import subprocess
+    from hsi_dmgasr_amd import _lib
+    structs = {"hsidm_attn_desc": _lib.AttnDesc, "hsidm_rope_desc": _lib.RopeDesc, "hsidm_tensor_item": _lib.TensorItem}
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "hsidm.h"', 'int main(void) {', 'printf("%zu\\n", sizeof(hsidm_attn_tile));']
+    for name, s in structs.items():
+        lines.append('printf("%%zu\\n", sizeof(%s));' % name)
+        lines += ['printf("%%zu\\n", offsetof(%s, %s));' % (name, f) for f, _ in s._fields_]
+    src = tmp_path / "probe.c"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "probe")])
+    got = list(map(int, subprocess.check_output([str(tmp_path / "probe")]).split()))
+    want = [16]
+    for s in structs.values():
+        want += [ctypes.sizeof(s)] + [getattr(s, f).offset for f, _ in s._fields_]
+    assert got == want
+
+
 # ------------------------------------------------------------------------------------------------------------------- GPU
 CASES = [  # lengths, hq, hk, D, causal
     ([1], 1, 1, 64, True), ([1, 1, 1], 2, 1, 32, False), ([31, 1, 64, 7, 103], 8, 2, 64, True), ([33, 0, 65, 129], 4, 4, 128, True),
     ([200, 3, 0], 2, 2, 40, False), ([257, 255], 3, 1, 96, True), ([128, 127, 64], 6, 2, 256, False), ([300, 70], 2, 1, 200, True),
     ([1025], 1, 1, 64, False), ([700, 5], 1, 1, 128, True), ([2049], 8, 1, 8, True), ([500, 400, 300, 200, 100], 16, 8, 16, False),
-    ([40] * 150, 8, 4, 64, True), ([1300], 2, 2, 256, True),
+    ([40] * 150, 8, 4, 64, True), ([1300], 2, 2, 256, True), ([70, 3], 2, 1, 24, False), ([129], 5, 5, 56, True), ([64], 3, 3, 72, False),
 ]
 
 

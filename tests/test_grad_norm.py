@@ -185,6 +185,10 @@ def test_clip_refusals(dev):
     with pytest.raises(ValueError, match="overlap"):
         T.clip_grad_norm_([x[:33], x[32:]], 1.0)
     T.clip_grad_norm_([x[:32], x[32:]], 1.0)
+    w = torch.nn.Parameter(torch.ones(5, device=dev))
+    with pytest.raises(ValueError, match="p.grad"):
+        T.clip_grad_norm_([w], 1.0)
+    assert bool((w == 1).all())
     with pytest.raises(ValueError, match="dense"):
         T.grad_norm([x.view(8, 8)[:, :4]])
     with pytest.raises(TypeError):

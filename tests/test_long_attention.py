@@ -238,3 +238,24 @@ def test_sampler_over_long_maps(dev):
     a = gd.p_sample_loop_batched(cond)
     b = gd.p_sample_loop_batched(cond)
     assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+@GPU
+def test_copies_of_a_used_module(dev):
+    """copy.deepcopy and a pickle round trip of a layer that has run (an averaged copy of the network is a common one)."""
+    import copy
+    import io
+    from hsi_dmgasr_amd.sr3_modules import unet
+    m = unet.SelfAttention(64, n_head=2, qk_norm_rope=True).to(dev).eval()
+    m.precision = "fp32"
+    x = torch.from_numpy(synth_tensor("la.x", (1, 64, 36, 34))).to(dev)
+    with torch.no_grad():
+        want = m(x)
+        twin = copy.deepcopy(m)
+        buf = io.BytesIO()
+        torch.save(m, buf)
+        buf.seek(0)
+        loaded = torch.load(buf, weights_only=False)                # (written two lines above)
+        del m
+        torch.cuda.empty_cache()
+        assert torch.equal(twin(x), want) and torch.equal(loaded(x), want)
