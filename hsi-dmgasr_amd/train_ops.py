@@ -307,10 +307,6 @@ class TensorList:
         for t in tensors:
             if not torch.is_tensor(t) or t.layout != torch.strided:
                 raise TypeError("hsidm: gradients must be strided tensors, got %s" % type(t).__name__)
-            if not t.is_cuda:
-                raise RuntimeError("hsidm: tensor is on %s; the HIP path needs a ROCm device tensor" % t.device)
-        if len({t.device for t in tensors}) > 1:
-            raise ValueError("hsidm: the tensors of one gradient norm must be on one device")
         self.tensors = tensors
         self.device = tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
         self._key, self._items, self._disjoint = None, None, None
@@ -323,6 +319,10 @@ class TensorList:
         if key != self._key:
             arr = (_lib.TensorItem * max(1, len(ts)))()
             for it, t in zip(arr, ts):
+                if not t.is_cuda:
+                    raise RuntimeError("hsidm: tensor is on %s; the HIP path needs a ROCm device tensor" % t.device)
+                if t.device != self.device:
+                    raise ValueError("hsidm: the tensors of one gradient norm must be on one device")
                 if t.numel() and not _is_dense(t):
                     raise ValueError("hsidm: a gradient of shape %s with strides %s is not dense" % (tuple(t.shape), t.stride()))
                 it.ptr, it.n, it.type = t.data_ptr(), t.numel(), _lib.type_id(t.dtype)

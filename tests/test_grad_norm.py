@@ -210,6 +210,9 @@ def test_list_follows_new_storage(dev):
     assert float(T.grad_norm(tl)) == 10.0
     x.data = torch.full((400,), 2.0, device=dev)
     assert float(T.grad_norm(tl)) == 40.0
+    x.data = torch.ones(7)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        T.grad_norm(tl)
 
 
 @GPU
