@@ -633,11 +633,11 @@ def _check_rope(q, k, wq, wk, pos, axes, eps):
         raise ValueError("hsidm: positions must be int32 [%d, %d], got %s %s" % (T, len(axes.sections), pos.dtype, tuple(pos.shape)))
     if any(t.device != q.device for t in (k, wq, wk, pos, axes.freq)):
         raise ValueError("hsidm: q, k, weights, positions and axes must be on one device")
-    if not float(eps) >= 0:
+    if not eps >= 0:
         raise ValueError("hsidm: eps must not be negative, got %r" % (eps,))
     base(q)
     d = _lib.RopeDesc()
-    d.T, d.Hq, d.Hk, d.D, d.axes, d.prec, d.eps = T, Hq, k.shape[1], D, len(axes.sections), tid, float(eps)
+    d.T, d.Hq, d.Hk, d.D, d.axes, d.prec, d.eps = T, Hq, k.shape[1], D, len(axes.sections), tid, eps
     d.freq = axes.freq.data_ptr()
     for i, n in enumerate(axes.sections):
         d.sections[i] = n
@@ -656,6 +656,7 @@ def _check_rope(q, k, wq, wk, pos, axes, eps):
 def rope_desc(q, k, wq, wk, pos, axes, eps):
     """(descriptor, backward workspace bytes, tensors it points into) of hsidm_qk_norm_rope.  The checks of a combination of shapes,
     strides, types and devices are made once per RotaryAxes; the addresses are each call's own."""
+    eps = float(eps)
     key = (q.shape, k.shape, wq.shape, wk.shape, pos.shape, q.stride(), k.stride(), wq.stride(), wk.stride(), pos.stride(), q.dtype, k.dtype, wq.dtype,
            wk.dtype, pos.dtype, q.device, k.device, wq.device, wk.device, pos.device, eps)
     plan = axes._plans.get(key)
@@ -717,8 +718,11 @@ class PackedSequences:
                 parts.append(table[np.argsort(-w, kind="stable")])
             setattr(self, "n%d" % rows, len(seq))
         self._tables = torch.from_numpy(np.concatenate(parts)).to(device)
-        self.device = self._tables.device
         self._plans = {}                                  # (attn_desc)
+
+    @property
+    def device(self):                                     # (the tables': a copy may have been loaded to another)
+        return self._tables.device
 
     def __getstate__(self):                               # copies and pickles of a module that holds one: the plans point at this object's tables
         return {**self.__dict__, "_plans": {}}
@@ -749,12 +753,12 @@ def _check_attn(q, k, v, seqs, causal, scale):
         raise ValueError("hsidm: %d tokens, but the sequences have %d" % (T, seqs.total))
     if any(t.device != q.device for t in (k, v)) or seqs.device != q.device:
         raise ValueError("hsidm: q, k, v and the sequences must be on one device")
-    scale = D ** -0.5 if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else scale
     if not 0.0 < scale < 1e30:
         raise ValueError("hsidm: scale must be positive, got %r" % (scale,))
     base(q)
     d = _lib.AttnDesc()
-    d.T, d.Hq, d.Hk, d.D, d.prec, d.causal, d.scale = T, Hq, Hk, D, tid, int(bool(causal)), scale
+    d.T, d.Hq, d.Hk, d.D, d.prec, d.causal, d.scale = T, Hq, Hk, D, tid, int(causal), scale
     kinds = ("causal q", "causal k") if causal else ("full", "full")
     d.qtiles64, d.qtiles128 = (seqs._tiles(kinds[0], r) for r in (64, 128))
     d.ktiles64, d.ktiles128 = (seqs._tiles(kinds[1], r) for r in (64, 128))
@@ -775,6 +779,7 @@ def _check_attn(q, k, v, seqs, causal, scale):
 def attn_desc(q, k, v, seqs, causal, scale):
     """(descriptor, forward workspace bytes, backward workspace bytes, tensors it points into) of hsidm_attention_packed.  The checks of
     a combination of shapes, strides, types and devices are made once per PackedSequences; the addresses are each call's own."""
+    causal, scale = bool(causal), None if scale is None else float(scale)
     key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device, v.device, causal, scale)
     plan = seqs._plans.get(key)
     if plan is None:

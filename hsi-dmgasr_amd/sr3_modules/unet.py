@@ -271,6 +271,9 @@ class SelfAttention(_HipModule):
         self._cache = _PackCache()
         self._maps = {}
 
+    def __getstate__(self):                            # (copies and checkpoints make their own plans, where they are)
+        return {**self.__dict__, "_maps": {}}
+
     def packed(self, tokens):
         """Does a map of that many tokens run on the packed attention kernels?"""
         return self.qk_norm_rope or tokens > 1024

@@ -229,13 +229,13 @@ int hsidm_attention(int prec, const void* qkv, void* out, int B, int N, int C, v
  * softmax and sums in fp32, probabilities rounded to the type ahead of their product with v.
  * Tiles (device memory, built by the caller once per set of lengths): for tile heights 64 and 128, the row ranges of every sequence of one
  * or more tokens - {first token of the sequence, its length, first row of the tile within it, 0} - n64 / n128 of them; qtiles: in the
- * order query tiles should start (most work first), ktiles: key tiles.  longest: the longest sequence.  Rows that no tile covers are not
- * written.
+ * order query tiles should start (most work first), ktiles: key tiles.  longest: the longest sequence.  The
+ * tiles together cover every one of the T tokens (what a split leaves in a row that none covers is undefined).
  * Values of k and v must be finite where a LATER token of the same 128-row tile is masked out for an earlier one (0 * inf is NaN).
  * out_lo (16-bit types; may be NULL): what rounding out to the type left behind, for the backward pass: rowsum(dout o out) from both is
  *   exact to fp32, and dq / dk are then as exact as rounding dS allows.
  * Backward: from out (+ out_lo), lse and dout, recomputing the scores: dq, dk, dv (strided like their tensors), dk / dv summed over the heads that
- * share them; no atomics, fixed order.  Workspaces: the _workspace_bytes functions (forward: 0 unless the keys are split), 16-byte aligned. */
+ * share them; no atomics, fixed order (fp16: P and dS are scaled by one power of two per call, from the largest |dout|^2 |v|^2).  Workspaces: the _workspace_bytes functions (forward: 0 unless the keys are split), 16-byte aligned. */
 typedef struct hsidm_attn_tile { int32_t start, len, row0, reserved; } hsidm_attn_tile;
 typedef struct hsidm_attn_desc {
     const void *q, *k, *v;

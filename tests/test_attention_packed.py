@@ -159,6 +159,19 @@ def test_structs_match_the_header(tmp_path):
     assert got == want
 
 
+def test_loaded_to_another_device():
+    """The sequences say where their tables ARE: the descriptor would otherwise pass addresses of another memory."""
+    import io
+    from hsi_dmgasr_amd import ops
+    s = ops.PackedSequences([3, 70], device="cpu")
+    s._plans["x"] = 1
+    buf = io.BytesIO()
+    torch.save(s, buf)
+    buf.seek(0)
+    loaded = torch.load(buf, map_location="meta", weights_only=False)          # (written three lines above)
+    assert s.device.type == "cpu" and loaded.device.type == "meta" and loaded.lengths == s.lengths and not loaded._plans
+
+
 # ------------------------------------------------------------------------------------------------------------------- GPU
 CASES = [  # lengths, hq, hk, D, causal
     ([1], 1, 1, 64, True), ([1, 1, 1], 2, 1, 32, False), ([31, 1, 64, 7, 103], 8, 2, 64, True), ([33, 0, 65, 129], 4, 4, 128, True),
@@ -307,6 +320,24 @@ def test_layouts(dev, layout):
         Tr.attention_packed_bwd(do, q, k, v, o, (saved.lse[:, :-1], None), seqs)
     with pytest.raises(ValueError, match="like q"):
         Tr.attention_packed_bwd(do[:-1], q, k, v, o, saved, seqs)
+
+
+@GPU
+def test_scalar_arguments_are_read_on_every_call(dev):
+    """scale and eps given as tensors that the caller rewrites in place."""
+    from hsi_dmgasr_amd import ops
+    q, k, v = torch.randn(3, 40, 2, 32, generator=torch.Generator().manual_seed(3)).to(dev)
+    seqs, s = ops.PackedSequences([40], device=dev), torch.tensor(0.5)
+    a = ops.attention_packed(q, k, v, seqs, scale=s)
+    s.fill_(2.0)
+    b = ops.attention_packed(q, k, v, seqs, scale=s)
+    assert torch.equal(a, ops.attention_packed(q, k, v, seqs, scale=0.5)) and torch.equal(b, ops.attention_packed(q, k, v, seqs, scale=2.0))
+    assert not torch.equal(a, b)
+    axes, w, pos, eps = ops.RotaryAxes((4,), 32, device=dev), torch.ones(32, device=dev), torch.zeros(40, 1, dtype=torch.int32, device=dev), torch.tensor(0.5)
+    a = ops.qk_norm_rope(q, k, w, w, pos, axes, eps=eps)[0]
+    eps.fill_(2.0)
+    b = ops.qk_norm_rope(q, k, w, w, pos, axes, eps=eps)[0]
+    assert torch.equal(b, ops.qk_norm_rope(q, k, w, w, pos, axes, eps=2.0)[0]) and not torch.equal(a, b)
 
 
 @GPU
