@@ -126,7 +126,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(RopeShape s, Rope
                 float ss = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) ss += a[j] * a[j] + b[j] * b[j];
-                const float r = rsqrtf(group_sum(ss, s.group) / (float)s.D + s.eps);
+                float r = rsqrtf(group_sum(ss, s.group) / (float)s.D + s.eps);
+                r = token < s.T ? r : 0.f;               // (behind the last token the row is zeros: with eps = 0, 0 * infinity)
                 float dot = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {

@@ -126,6 +126,28 @@ def test_forward_and_backward(dev, case, dtype):
 
 
 @GPU
+@pytest.mark.parametrize("T, D", [(1, 16), (5, 64), (67, 48), (3, 256)])
+def test_no_eps(dev, T, D):
+    """eps = 0 is allowed where no row is zero: the lanes behind the last token, which hold zeros, must not reach the weights' gradients."""
+    from hsi_dmgasr_amd import ops
+    from hsi_dmgasr_amd import train_ops as Tr
+    q, k, wq, wk, pos = inputs(dev, T, 2, 1, D, 1, torch.float32, seed=4)
+    axes = ops.RotaryAxes((D // 4,), D, device=dev)
+    outs = ops.qk_norm_rope(q, k, wq, wk, pos, axes, eps=0.0)
+    g = torch.Generator().manual_seed(9)
+    do = torch.randn(T, 2, D, generator=g).to(dev), torch.randn(T, 1, D, generator=g).to(dev)
+    grads = Tr.qk_norm_rope_bwd(*do, q, k, wq, wk, pos, axes, eps=0.0)
+    for x, w, o, d, dx, dw in ((q, wq, outs[0], do[0], grads[0], grads[2]), (k, wk, outs[1], do[1], grads[1], grads[3])):
+        x64, w64 = x.double().requires_grad_(), w.double().requires_grad_()
+        y = plain64(x64, w64, pos, (D // 4,), 0.0)
+        close(o, y.detach())
+        y.backward(d.double())
+        close(dx, x64.grad, terms=4)
+        mag = plain64(x.double().abs(), torch.ones_like(w64), pos * 0, (D // 4,), 0.0).mul(d.double().abs().amax()).sum((0, 1))
+        assert bool(((dw.double() - w64.grad).abs() <= 64 * 2.0 ** -24 * mag + 1e-30).all())        # (the bound of test_forward_and_backward)
+
+
+@GPU
 def test_gradient_against_differences(dev):
     """d loss / d x along random directions, by central differences of the forward kernel in fp32 (loss = sum of out * do)."""
     from hsi_dmgasr_amd import ops
