@@ -402,7 +402,7 @@ def qk_norm_rope_bwd(d_out_q, d_out_k, q, k, wq, wk, pos, axes, eps=1e-6, out=No
 def attention_packed_bwd(do, q, k, v, out, saved, seqs, causal=False, scale=None, grads=None):
     """Gradient of ops.attention_packed: (dq, dk, dv) in the inputs' type from the output's gradient do, the inputs, the output and what
     the forward pass saved (its AttentionSaved).  grads: optional (dq, dk, dv) to write into, [T, H, D] views with 16-byte aligned rows
-    (slices of a dqkv)."""
+    (slices of a dqkv) that share no element with each other or with what is read."""
     d, _, nb, keep = ops.attn_desc(q, k, v, seqs, causal, scale)
     shape, dtype, dev = q.shape, q.dtype, q.device
     T, Hq, D = shape
