@@ -372,13 +372,14 @@ template <> struct GradScale<f16> {
     static constexpr bool on = true;
     static constexpr float p_shift = 10.f, p_back = 1.f / 1024.f;
 };
-// the power of two that dS = P' (dP - delta), P' = 2^10 P, is multiplied by
+// The power of two that dS = P' (dP - delta), P' = 2^10 P, is multiplied by.  The maxima are those of finite fp16 rows: at most 256 * 65504^2,
+// so that `top` is finite; it is zero only where every finite row of dO or of V is zero, and dS then is too.
 __device__ __forceinline__ float grad_factor(const float* maxima, int n, int lane) {
     float a = 0.f, b = 0.f;
     for (int i = lane; i < n; i += 64) { a = fmaxf(a, maxima[2 * i]); b = fmaxf(b, maxima[2 * i + 1]); }
     a = wave_max(a); b = wave_max(b);
     const float top = 2048.f * sqrtf(a) * sqrtf(b);              // |P' (dP - delta)|
-    if (!(top > 0.f) || !(top < 1e30f)) return 1.f;
+    if (!(top > 0.f)) return 1.f;
     int e;
     frexpf(32768.f / top, &e);
     e = max(min(e - 1, 60), -60);

@@ -66,9 +66,12 @@ __global__ __launch_bounds__(256) void attn_add_kernel(AttnSums sums, int64_t T_
 }
 
 // delta[h][t] = sum_d dO O per row, O with its rounding residual where the forward pass kept it (without it, delta's error is as large as
-// that of rounding dS and adds to it in dQ and dK: 1.55 ... 1.7 instead of 1.4 times the output's own rounding); fp16: also this workgroup's largest |dO|^2 and |V|^2 (GradScale).  `group` lanes, a power of two that
-// covers a row's 16-byte pieces, share a row.
+// that of rounding dS and adds to it in dQ and dK: 1.55 ... 1.7 instead of 1.4 times the output's own rounding); fp16: also this workgroup's largest |dO|^2 and |V|^2 (GradScale) of
+// its finite rows - a row with an infinity or a NaN has no finite gradient to scale, and must not decide the scale of the others'.
+// `group` lanes, a power of two that covers a row's 16-byte pieces, share a row.
 constexpr int kDeltaBlocks = 512;
+
+__device__ __forceinline__ float finite_or_zero(float x) { return x < INFINITY ? x : 0.f; }      // (of a sum of squares: NaN compares false)
 
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTensor o, const char* __restrict__ lo, AttnTensor v, int64_t T_, int Hq, int Hk, int pieces, int group,
@@ -98,7 +101,7 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTe
             }
         }
         dot = sum(dot);
-        if (GradScale<T>::on) ma = fmaxf(ma, sum(sq));
+        if (GradScale<T>::on) ma = fmaxf(ma, finite_or_zero(sum(sq)));
         if (r < T_ * Hq && sub == 0) delta[head * T_ + token] = dot;
     }
     if constexpr (GradScale<T>::on) {
@@ -111,7 +114,7 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTe
 #pragma unroll
                 for (int k = 0; k < E; ++k) sq += (float)x[k] * (float)x[k];
             }
-            mb = fmaxf(mb, sum(sq));
+            mb = fmaxf(mb, finite_or_zero(sum(sq)));
         }
         ma = wave_max(ma); mb = wave_max(mb);
         if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = ma; red[1][threadIdx.x >> 6] = mb; }
