@@ -234,9 +234,15 @@ struct AttnFwdArgs {
     float scale;
 };
 
+// How a probability is held ahead of its product with V: times 2^shift, the row's largest between 2^shift and 2^(shift + lazy).  bf16 and
+// fp32 have the exponents for any row.  fp16 rounds what is below 2^-14 to steps of 2^-24: at scale one, keys at 2^-26 of the largest would
+// vanish from the sum (a thousandth of a row of 65536 of them) and stay in the softmax's denominator.  Held between 2^11 and 2^15 (65504 is
+// the largest fp16) half a step is 2^-36 of the largest: 2^25 keys lose less than the output's rounding.
+template <typename T> struct ProbScale { static constexpr float shift = 0.f, lazy = 8.f, back = 1.f; };
+template <> struct ProbScale<f16> { static constexpr float shift = 11.f, lazy = 4.f, back = 1.f / 2048.f; };
+
 // O^T = V^T P^T with the softmax's running maximum and sum per column (= query = lane).  The maximum that scales the accumulators
-// follows the true one lazily: only when some query's grew by more than 2^8 are they rescaled (fp16 probabilities stay below 2^8, sums
-// are fp32 in any case).  NW waves of 32 queries each walk the key tiles together; two LDS buffers: a tile arrives while the one
+// follows the true one lazily: only when some query's grew by more than 2^lazy (ProbScale) are they rescaled; sums are fp32 in any case.  NW waves of 32 queries each walk the key tiles together; two LDS buffers: a tile arrives while the one
 // before it is multiplied.
 // Bound by the matrix pipe and the exponentials beside it (at D = 64 the vector unit has 680 cycles of work per 512 of the matrix pipe's).
 // fp16, 2 x 16384 tokens, one head of 64: 188 us, 730 TFLOP/s; bf16 causal, 20115 tokens in six sequences, 16 / 4 heads of 128: 515 us, 905
@@ -300,7 +306,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 512 ? 2 : 1)) void a
 #pragma unroll
                 for (int j = 0; j < 16; ++j) mt = fmaxf(mt, s[b][j]);
             mt = both_halves_max(mt);
-            if (!SKIP || __any(!((mt - m) * c <= 8.0f) && mt != -INFINITY)) {
+            if (!SKIP || __any(!((mt - m) * c <= ProbScale<T>::lazy) && mt != -INFINITY)) {
                 const float mn = fmaxf(m, mt), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
                 m = mn;
                 l *= f;
@@ -309,7 +315,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 512 ? 2 : 1)) void a
 #pragma unroll
                     for (int j = 0; j < 16; ++j) o[d][j] *= f;
             }
-            const float mc = m == -INFINITY ? 0.f : m * c;
+            const float mc = (m == -INFINITY ? 0.f : m * c) - ProbScale<T>::shift;
             ColFrag<T> p[BN / 32];
 #pragma unroll
             for (int b = 0; b < BN / 32; ++b) {
@@ -343,7 +349,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 512 ? 2 : 1)) void a
             for (int d = 0; d < ND; ++d) store_residual<T>(lo, o[d], inv, 32 * d, h, a.D);
         }
     }
-    if (a.lse && h == 0) a.lse[((int64_t)blockIdx.y * a.Hq + head) * a.T + token] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+    if (a.lse && h == 0) a.lse[((int64_t)blockIdx.y * a.Hq + head) * a.T + token] = l == 0.f ? -INFINITY : m * a.scale + logf(l * ProbScale<T>::back);
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------

@@ -1,10 +1,11 @@
-"""Packed attention where fp16's five exponent bits matter: gradients next to a sequence that holds infinities."""
+"""Packed attention where fp16's eleven bits and five exponent bits matter: probabilities far below a row's largest one, and gradients next
+to a sequence that holds infinities."""
 import math
 
 import pytest
 import torch
 
-from test_attention_packed import close, make, plain64
+from test_attention_packed import SCORES, close, make, plain64
 
 GPU = pytest.mark.gpu
 
@@ -12,6 +13,35 @@ GPU = pytest.mark.gpu
 @pytest.fixture(scope="module")
 def dev():
     return torch.device("cuda:0")
+
+
+@GPU
+@pytest.mark.parametrize("dominant", ["first", "last"])
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16, torch.float32], ids=str)
+def test_many_keys_far_below_the_largest(dev, kind, dominant):
+    """One key with a score of 18 among 65536 at zero, the same for every query: each of them has e^-18 = 2^-26 of its probability, together
+    they are 2^-10 of the row, and they are all there is of the output's first half (the dominant key's values are zero there)."""
+    from hsi_dmgasr_amd import ops
+    n, D = 65537, 64
+    at = 0 if dominant == "first" else n - 1
+    q, k = torch.zeros(n, 1, D), torch.zeros(n, 1, D)
+    q[:, :, 0], k[at, :, 0] = 1.0, 18.0
+    v = torch.rand(n, 1, D, generator=torch.Generator().manual_seed(11)) + 0.5
+    v[at, :, :32] = 0.0
+    q, k, v = (t.to(kind).to(dev) for t in (q, k, v))
+    seqs = ops.PackedSequences([n], device=dev)
+    o, saved = ops.attention_packed(q, k, v, seqs, scale=1.0, want_lse=True)
+    p = torch.exp(k[:, 0, 0].double() - 18.0)
+    p = p / p.sum()
+    want = p @ v[:, 0].double()                                     # (no negative value: a sum of magnitudes too)
+    # the store's half step; a probability's half step, where the type has it as a normal number; below that half a subnormal step - the
+    # scale is such that a row's largest probability is between 2^11 and 2^15, so 2^-25 is 2^-36 of it; and fp32 scores, exponentials, sums
+    u = torch.finfo(kind).eps / 2
+    tol = want * u + want * (0 if kind == torch.float32 else u) + want * SCORES * 2.0 ** -24
+    if kind == torch.float16:
+        tol = tol + 2.0 ** -36 * v[:, 0].double().sum(0)
+    assert bool(((o.double() - want).abs() <= tol).all()), float(((o.double() - want).abs() / tol).max())
+    assert float((saved.lse.double() - (18.0 + math.log1p((n - 1) * math.exp(-18.0)))).abs().max()) <= SCORES * 2.0 ** -24 * 2
 
 
 @GPU
