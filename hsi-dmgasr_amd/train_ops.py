@@ -294,13 +294,13 @@ def _is_dense(t):
     return True
 
 
-_data_ptr, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
+_data_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
 
 
 class TensorList:
     """The tensors of a gradient norm or clipping call, checked once: dense fp32 / bf16 / fp16 ROCm tensors of one device, mixed types
     as they come (None entries - parameters without a gradient - are left out).  A program that keeps its gradient tensors keeps the
-    list too; addresses, sizes and types are read again on every call, so tensors that were given new storage are followed."""
+    list too; addresses, sizes, types and layouts are read again on every call, so tensors that were given new storage are followed."""
 
     def __init__(self, tensors):
         tensors = [tensors] if torch.is_tensor(tensors) else [t for t in tensors if t is not None]
@@ -313,9 +313,12 @@ class TensorList:
         self.items()
 
     def items(self):
-        """The host array of hsidm_grad_norm, made again where a tensor's address, size or type is another."""
+        """The host array of hsidm_grad_norm, made again where a tensor's address, size, type or layout is another."""
         ts = self.tensors
-        key = (list(map(_data_ptr, ts)), list(map(_numel, ts)), [t.dtype for t in ts])
+        flat = list(map(_contiguous, ts))                 # (a contiguous tensor's elements are the numel() from its address on: its strides add nothing)
+        key = (list(map(_data_ptr, ts)), list(map(_numel, ts)), [t.dtype for t in ts], flat)
+        if not all(flat):
+            key += ([(t.shape, t.stride()) for t, c in zip(ts, flat) if not c],)
         if key != self._key:
             arr = (_lib.TensorItem * max(1, len(ts)))()
             for it, t in zip(arr, ts):
@@ -367,7 +370,7 @@ def clip_grad_norm_(tensors, max_norm):
         raise ValueError("hsidm: clip_grad_norm_ needs tensors that do not overlap (is one of them listed twice?)")
     out = clip_coef(tl, max_norm)
     with _lib.on_device(tl.device):
-        _check(_lib.lib().hsidm_scale_tensors(tl.items(), len(tl.tensors), _lib.ptr(out) + 4, _lib.stream_ptr()), "scale_tensors")
+        _check(_lib.lib().hsidm_scale_tensors(tl._items, len(tl.tensors), _lib.ptr(out) + 4, _lib.stream_ptr()), "scale_tensors")
     written = [t for t in tl.tensors if not t.is_inference()]
     if written:
         torch.autograd.graph.increment_version(written)         # written through raw pointers
