@@ -597,7 +597,8 @@ def _strides(t):
 class RotaryAxes:
     """Frequencies of a rotary embedding over several position axes (time or band group, row, column): sections[a] pairs of every head turn
     with axis a, pair j of them by base^(-j / sections[a]) radians per position; pairs beyond sum(sections) (at most D/2) are not turned.
-    Pair p of a head is its elements (p, p + D/2).  The table is built once, in 64 bits."""
+    Pair p of a head is its elements (p, p + D/2).  The table, freq (turns per position, fp64), is built once, in 64 bits; another one of
+    that kind may take its place between calls (rescaled frequencies)."""
 
     def __init__(self, sections, head_dim, base=10000.0, device="cuda"):
         self.sections = tuple(int(n) for n in sections)
@@ -631,6 +632,10 @@ def _check_rope(q, k, wq, wk, pos, axes, eps):
             raise ValueError("hsidm: norm weights must be fp32 [%d], got %s %s" % (D, w.dtype, tuple(w.shape)))
     if pos.dtype != torch.int32 or tuple(pos.shape) != (T, len(axes.sections)):
         raise ValueError("hsidm: positions must be int32 [%d, %d], got %s %s" % (T, len(axes.sections), pos.dtype, tuple(pos.shape)))
+    if not 1 <= len(axes.sections) <= 4 or min(axes.sections) < 0 or sum(axes.sections) > D // 2:
+        raise ValueError("hsidm: one to four axes with non-negative sections of at most %d pairs together, got %r" % (D // 2, axes.sections))
+    if axes.freq.dtype != torch.float64 or axes.freq.dim() != 1 or not axes.freq.is_contiguous() or axes.freq.numel() < max(1, sum(axes.sections)):
+        raise ValueError("hsidm: freq must be a contiguous fp64 table of %d frequencies, got %s %s" % (sum(axes.sections), axes.freq.dtype, tuple(axes.freq.shape)))
     if any(t.device != q.device for t in (k, wq, wk, pos, axes.freq)):
         raise ValueError("hsidm: q, k, weights, positions and axes must be on one device")
     if not eps >= 0:
@@ -638,12 +643,11 @@ def _check_rope(q, k, wq, wk, pos, axes, eps):
     base(q)
     d = _lib.RopeDesc()
     d.T, d.Hq, d.Hk, d.D, d.axes, d.prec, d.eps = T, Hq, k.shape[1], D, len(axes.sections), tid, eps
-    d.freq = axes.freq.data_ptr()
     for i, n in enumerate(axes.sections):
         d.sections[i] = n
     nb = 0
     if T:
-        d.q = d.k = d.wq = d.wk = d.pos = d.freq & ~15        # (any aligned address: the size does not depend on it)
+        d.q = d.k = d.wq = d.wk = d.pos = d.freq = 64          # (any aligned address: the size does not depend on it)
         nb = _lib.lib().hsidm_qk_norm_rope_bwd_workspace_bytes(C.byref(d))
         if nb < 0:
             _lib.check(int(nb), "qk_norm_rope_bwd_workspace_bytes")
@@ -656,9 +660,10 @@ def _check_rope(q, k, wq, wk, pos, axes, eps):
 def rope_desc(q, k, wq, wk, pos, axes, eps):
     """(descriptor, backward workspace bytes, tensors it points into) of hsidm_qk_norm_rope.  The checks of a combination of shapes,
     strides, types and devices are made once per RotaryAxes; the addresses are each call's own."""
-    eps = float(eps)
+    eps, freq = float(eps), axes.freq
     key = (q.shape, k.shape, wq.shape, wk.shape, pos.shape, q.stride(), k.stride(), wq.stride(), wk.stride(), pos.stride(), q.dtype, k.dtype, wq.dtype,
-           wk.dtype, pos.dtype, q.device, k.device, wq.device, wk.device, pos.device, eps)
+           wk.dtype, pos.dtype, q.device, k.device, wq.device, wk.device, pos.device, eps, axes.head_dim, tuple(axes.sections), freq.shape,
+           freq.dtype, freq.device, freq.is_contiguous())
     plan = axes._plans.get(key)
     if plan is None:
         plan = _check_rope(q, k, wq, wk, pos, axes, eps)
@@ -672,8 +677,8 @@ def rope_desc(q, k, wq, wk, pos, axes, eps):
         ptrs = [t.data_ptr() for t in (q, k, wq, wk)]
         (d.q_ts, d.q_hs), (d.k_ts, d.k_hs) = _strides(q), _strides(k)
     d.q, d.k, d.wq, d.wk = ptrs
-    d.pos = pos.data_ptr()
-    return d, plan[1], (q, k, wq, wk, pos)
+    d.pos, d.freq = pos.data_ptr(), freq.data_ptr()
+    return d, plan[1], (q, k, wq, wk, pos, freq)
 
 
 def _aligned(t):
