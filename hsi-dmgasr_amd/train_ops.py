@@ -397,8 +397,8 @@ def qk_norm_rope_bwd(d_out_q, d_out_k, q, k, wq, wk, pos, axes, eps=1e-6, out=No
     with _lib.on_device(q.device):
         ws = q.new_empty(nb, dtype=torch.uint8)
         gq, gk = ops._aligned(d_out_q), ops._aligned(d_out_k)
-        _check(L.hsidm_qk_norm_rope_bwd(C.byref(d), gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0),
-                                        dk.stride(1), dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), nb, _lib.stream_ptr()), "qk_norm_rope_bwd")
+        _check(L.hsidm_qk_norm_rope_bwd(C.byref(d), gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), *ops._strides(dq), dk.data_ptr(),
+                                        *ops._strides(dk), dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), nb, _lib.stream_ptr()), "qk_norm_rope_bwd")
     return dq, dk, dwq, dwk
 
 

@@ -57,3 +57,21 @@ def test_rescaled_frequencies(dev):
     assert torch.equal(b, ops.qk_norm_rope(q, q, w, w, pos, twin)[0]) and not torch.equal(a, b)
     # (half an fp64 frequency at twice a position is the same 64-bit angle)
     assert abs(float(axes.freq[0]) * 2 * math.pi - 0.5) < 1e-15
+
+
+@GPU
+@pytest.mark.parametrize("T, H", [(1, 2), (3, 1), (1, 1)])
+def test_outputs_with_an_axis_of_length_one(dev, T, H):
+    """The stride of an axis of length one is any number (torch leaves it to the view): it is no reason to refuse an output."""
+    from hsi_dmgasr_amd import ops
+    from hsi_dmgasr_amd import train_ops as Tr
+    g = torch.Generator().manual_seed(2)
+    q, dq, k, dk = (torch.randn(T, H, 64, generator=g).to(dev) for _ in range(4))
+    w, pos = torch.ones(64, device=dev), torch.arange(T, dtype=torch.int32, device=dev)[:, None]
+    axes = ops.RotaryAxes((16,), 64, device=dev)
+    want = Tr.qk_norm_rope_bwd(dq, dk, q, k, w, w, pos, axes)
+    strides = (13 if T == 1 else 64 * H, 7 if H == 1 else 64, 1)
+    out = tuple(torch.zeros(T * H * 64, device=dev).as_strided((T, H, 64), strides) for _ in range(2))
+    assert all(ops.rows_aligned(o) for o in out)
+    got = Tr.qk_norm_rope_bwd(dq, dk, q, k, w, w, pos, axes, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0] is out[0] and got[1] is out[1]
