@@ -583,6 +583,13 @@ def rows_aligned(t):
     return t.data_ptr() % 16 == 0 and rows_strided(t)
 
 
+def rows_apart(t):
+    """Do no two (token, head) rows of [T, H, D] share an element (an output's must not)?"""
+    (a, b, _), (n, h, d) = t.stride(), t.shape
+    a, b = a if n > 1 else d, b if h > 1 else d
+    return n * h == 0 or min(a, b) >= d and (a >= (h - 1) * b + d or b >= (n - 1) * a + d)
+
+
 def token_rows(t):
     """t itself where the kernels can address its rows, else a contiguous copy (odd offsets or strides, a transposed last axis)."""
     return t if rows_aligned(t) else t.contiguous() if t.data_ptr() % 16 == 0 or not t.is_contiguous() else t.clone()

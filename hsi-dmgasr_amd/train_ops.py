@@ -388,8 +388,8 @@ def qk_norm_rope_bwd(d_out_q, d_out_k, q, k, wq, wk, pos, axes, eps=1e-6, out=No
             raise ValueError("hsidm: a gradient of %s %s does not belong to a tensor of %s %s" % (tuple(g.shape), g.dtype, tuple(x.shape), x.dtype))
     dq, dk = (q.new_empty(q.shape), k.new_empty(k.shape)) if out is None else out
     for g, x in () if out is None else ((dq, q), (dk, k)):
-        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device or not ops.rows_aligned(g):
-            raise ValueError("hsidm: out must be [T, H, D] tensors like q and k with 16-byte aligned rows")
+        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device or not ops.rows_aligned(g) or not ops.rows_apart(g):
+            raise ValueError("hsidm: out must be [T, H, D] tensors like q and k with 16-byte aligned rows that do not overlap")
     dwq, dwk = (torch.zeros if T == 0 else torch.empty)((2, D), dtype=torch.float32, device=q.device).unbind(0)
     if T == 0:
         return dq, dk, dwq, dwk
@@ -421,8 +421,8 @@ def attention_packed_bwd(do, q, k, v, out, saved, seqs, causal=False, scale=None
         strides = ((Hq * D, D), (Hk * D, D), (Hk * D, D))
     else:
         for g, x in zip(grads, (q, k, v)):
-            if g.shape != x.shape or g.dtype != dtype or g.device != dev or not ops.rows_aligned(g):
-                raise ValueError("hsidm: grads must be [T, H, D] tensors like q, k, v with 16-byte aligned rows")
+            if g.shape != x.shape or g.dtype != dtype or g.device != dev or not ops.rows_aligned(g) or not ops.rows_apart(g):
+                raise ValueError("hsidm: grads must be [T, H, D] tensors like q, k, v with 16-byte aligned rows that do not overlap")
         strides = [ops._strides(g) for g in grads]
     dq, dk, dv = grads
     if T == 0:
