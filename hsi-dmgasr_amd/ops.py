@@ -572,6 +572,12 @@ def base(t):
     return t.data_ptr()
 
 
+def no_autograd(*tensors):
+    """The token operators' gradients are calls of their own (train_ops): a graph that would go through them is refused, not cut."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("hsidm: autograd does not record this call - run it under torch.no_grad() or on detached tensors, and call its gradient in train_ops")
+
+
 def rows_strided(t):
     """Are the (token, head) rows of [T, H, D] contiguous along D, whole multiples of 16 bytes apart, and tokens at most 16 MB?"""
     es, (a, b, c), (n, h, d) = t.element_size(), t.stride(), t.shape
@@ -696,7 +702,9 @@ def _aligned(t):
 def qk_norm_rope(q, k, wq, wk, pos, axes, eps=1e-6):
     """RMS norm of every query and key head (weights wq, wk fp32 [D]) and its rotation by the token's positions, one launch:
     q [T, Hq, D], k [T, Hk, D] (any strides; rows on 16-byte boundaries are read in place), pos int32 [T, axes], axes a RotaryAxes.
-    -> two contiguous tensors of q's type.  Gradient: train_ops.qk_norm_rope_bwd."""
+    -> two contiguous tensors of q's type.  Gradient: train_ops.qk_norm_rope_bwd (autograd does not record the call: refused where one
+    of q, k, wq, wk requires a gradient and gradients are enabled)."""
+    no_autograd(q, k, wq, wk)
     d, _, keep = rope_desc(q, k, wq, wk, pos, axes, eps)
     oq, ok = q.new_empty(q.shape), k.new_empty(k.shape)
     if d.T:
@@ -817,7 +825,9 @@ def attention_packed(q, k, v, seqs, causal=False, scale=None, want_lse=False):
     """softmax(scale * q k^T) v within every sequence of a packed batch: q [T, Hq, D], k / v [T, Hk, D] (Hk divides Hq; any strides, rows
     on 16-byte boundaries are read in place), seqs a PackedSequences over the T tokens; causal: a token sees itself and what came
     before; scale: 1/sqrt(D) unless given.  Any length - nothing of size length^2 is stored.  -> out [T, Hq, D] in q's type, with
-    want_lse also the AttentionSaved that train_ops.attention_packed_bwd takes (autograd does not record the call)."""
+    want_lse also the AttentionSaved that train_ops.attention_packed_bwd takes (autograd does not record the call: refused where one of q,
+    k, v requires a gradient and gradients are enabled)."""
+    no_autograd(q, k, v)
     d, nb, _, keep = attn_desc(q, k, v, seqs, causal, scale)
     out = q.new_empty(q.shape)
     lse = lo = None
