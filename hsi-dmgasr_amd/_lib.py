@@ -123,6 +123,7 @@ SIGNATURES = {
     "hsidm_gather_pack": [_vp, _vp, _i64, _vp, _vp, _vp],
     "hsidm_adam_step": [_vp, _vp, _vp, _vp, _i64, _f32, _f32, _f32, _f32, _i32, _f32, _vp, _vp],
     "hsidm_adam_step_clipped": [_vp, _vp, _vp, _vp, _i64, _f32, _f32, _f32, _f32, _i32, _f32, _vp, _vp, _vp],
+    "hsidm_adam_step_f64": [_vp, _vp, _vp, _vp, _i64, _f64, _f64, _f64, _f64, _i32, _f32, _vp, _vp, _vp],
     "hsidm_grad_norm_workspace_bytes": [_i32],
     "hsidm_grad_norm": [C.POINTER(TensorItem), _i32, _f64, _f64, _vp, _vp, _vp],
     "hsidm_scale_tensors": [C.POINTER(TensorItem), _i32, _vp, _vp],

@@ -475,13 +475,14 @@ __global__ __launch_bounds__(256) void noise_mlp_bwd_kernel(const float* __restr
 // memory sees four advancing fronts.  (4096 workgroups striding over the buffers, as this kernel ran first, touch 4096 places at once:
 // 600 us instead of 438 for 97.8 M parameters.)  The parameters and moments are not read again before the next step and go past the
 // caches (551 -> 511 us with the norm's 73).
+// rest = 1 - beta comes from the host, rounded from 64 bits (1.0f - 0.999f is 1.3e-5 off, and v is a sum of that times g^2).
 // BACK (a clipped step): from the buffers' end to their start - the norm has just read the gradient from start to end, and what it read
 // last is still in the 256 MB cache.
 template <bool BACK>
 __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
-                                                   float* __restrict__ v, int64_t n, float beta1, float beta2, float step_size,
-                                                   float inv_sqrt_bc2, float eps, float grad_scale, const float* __restrict__ coef,
-                                                   const float* __restrict__ clip) {
+                                                   float* __restrict__ v, int64_t n, float beta1, float rest1, float beta2, float rest2,
+                                                   float step_size, float inv_sqrt_bc2, float eps, float grad_scale,
+                                                   const float* __restrict__ coef, const float* __restrict__ clip) {
     if (clip) grad_scale *= clip[0];                                // hsidm_grad_norm's coefficient: the clipped gradient is never written
     if (coef) { step_size = coef[0]; inv_sqrt_bc2 = coef[1]; }      // a captured step: the bias corrections come from device memory
     const int64_t n4 = n >> 2, j = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -493,8 +494,8 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float gk = gg[k] * grad_scale;
-            mm[k] = beta1 * mm[k] + (1.0f - beta1) * gk;           // exp_avg.lerp_(grad, 1 - beta1)
-            vv[k] = beta2 * vv[k] + (1.0f - beta2) * gk * gk;      // exp_avg_sq.mul_(beta2).addcmul_(grad, grad, 1 - beta2)
+            mm[k] = beta1 * mm[k] + rest1 * gk;           // exp_avg.lerp_(grad, 1 - beta1)
+            vv[k] = beta2 * vv[k] + rest2 * gk * gk;      // exp_avg_sq.mul_(beta2).addcmul_(grad, grad, 1 - beta2)
             const float denom = sqrtf(vv[k]) * inv_sqrt_bc2 + eps;
             pp[k] -= step_size * (mm[k] / denom);
         }
@@ -505,8 +506,8 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const 
     if (blockIdx.x == 0 && threadIdx.x < (n & 3)) {
         const int64_t i = (n4 << 2) + threadIdx.x;
         const float gk = g[i] * grad_scale;
-        const float mk = beta1 * m[i] + (1.0f - beta1) * gk;
-        const float vk = beta2 * v[i] + (1.0f - beta2) * gk * gk;
+        const float mk = beta1 * m[i] + rest1 * gk;
+        const float vk = beta2 * v[i] + rest2 * gk * gk;
         m[i] = mk; v[i] = vk;
         p[i] -= step_size * (mk / (sqrtf(vk) * inv_sqrt_bc2 + eps));
     }
@@ -689,19 +690,25 @@ extern "C" int hsidm_gather_pack(const float* src, const int32_t* idx, int64_t n
     return (int)hipGetLastError();
 }
 
-extern "C" int hsidm_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
-                                       int step, float grad_scale, const float* coef_dev, const float* clip_dev, void* stream) {
+extern "C" int hsidm_adam_step_f64(float* p, const float* g, float* m, float* v, int64_t n, double lr, double beta1, double beta2, double eps,
+                                   int step, float grad_scale, const float* coef_dev, const float* clip_dev, void* stream) {
     if (!p || !g || !m || !v || n <= 0 || (step <= 0 && !coef_dev)) return HSIDM_E_BADARG;
     const int st = step > 0 ? step : 1;
-    const double bc1 = 1.0 - pow((double)beta1, st), bc2 = 1.0 - pow((double)beta2, st);
+    const double bc1 = 1.0 - pow(beta1, st), bc2 = 1.0 - pow(beta2, st);
     const int64_t blocks = ((n >> 2) + 255) / 256;
     if (blocks > 0x7fffffff) return HSIDM_E_UNSUPPORTED;
-    hipLaunchKernelGGL(clip_dev ? &adam_kernel<true> : &adam_kernel<false>, dim3((unsigned)(blocks > 0 ? blocks : 1)), dim3(256), 0, (hipStream_t)stream, p, g, m, v, n, beta1, beta2,
-                       (float)((double)lr / bc1), (float)(1.0 / sqrt(bc2)), eps, grad_scale, coef_dev, clip_dev);
+    hipLaunchKernelGGL(clip_dev ? &adam_kernel<true> : &adam_kernel<false>, dim3((unsigned)(blocks > 0 ? blocks : 1)), dim3(256), 0, (hipStream_t)stream, p, g, m, v, n,
+                       (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)(lr / bc1), (float)(1.0 / sqrt(bc2)), (float)eps,
+                       grad_scale, coef_dev, clip_dev);
     return (int)hipGetLastError();
+}
+
+extern "C" int hsidm_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
+                                       int step, float grad_scale, const float* coef_dev, const float* clip_dev, void* stream) {
+    return hsidm_adam_step_f64(p, g, m, v, n, lr, beta1, beta2, eps, step, grad_scale, coef_dev, clip_dev, stream);
 }
 
 extern "C" int hsidm_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
                                int step, float grad_scale, const float* coef_dev, void* stream) {
-    return hsidm_adam_step_clipped(p, g, m, v, n, lr, beta1, beta2, eps, step, grad_scale, coef_dev, nullptr, stream);
+    return hsidm_adam_step_f64(p, g, m, v, n, lr, beta1, beta2, eps, step, grad_scale, coef_dev, nullptr, stream);
 }

@@ -266,21 +266,17 @@ def gather_pack(src, idx, out_hi, out_lo=None):
 
 
 def adam_coefs(lr, beta1, beta2, step):
-    """(lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)): what hsidm_adam_step derives from `step`, for the device-resident form."""
+    """(lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)): what hsidm_adam_step_f64 derives from `step`, for the device-resident form."""
     return float(lr / (1.0 - beta1 ** step)), float(1.0 / (1.0 - beta2 ** step) ** 0.5)
 
 
 def adam_step(p, g, m, v, lr, beta1, beta2, eps, step, grad_scale=1.0, coef=None, clip=None):
     """coef: optional device tensor of two floats (adam_coefs) read by the kernel instead of deriving them from `step`.
     clip: optional result of clip_coef: the gradient enters scaled by its coefficient (and is not rewritten)."""
-    args = (_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), _lib.ptr(v), p.numel(), float(lr), float(beta1), float(beta2), float(eps), int(step),
-            float(grad_scale), _lib.ptr(coef))
-    if clip is None:
-        _check(_lib.lib().hsidm_adam_step(*args, _lib.stream_ptr()), "adam_step")
-        return
-    if clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or clip.device != p.device:
+    if clip is not None and (clip.dtype != torch.float32 or tuple(clip.shape) != (2,) or clip.device != p.device):
         raise ValueError("hsidm: clip must be clip_coef's fp32 [2] on the parameters' device")
-    _check(_lib.lib().hsidm_adam_step_clipped(*args, _lib.ptr(clip) + 4, _lib.stream_ptr()), "adam_step")
+    _check(_lib.lib().hsidm_adam_step_f64(_lib.ptr(p), _lib.ptr(g), _lib.ptr(m), _lib.ptr(v), p.numel(), float(lr), float(beta1), float(beta2), float(eps), int(step),
+                                          float(grad_scale), _lib.ptr(coef), None if clip is None else _lib.ptr(clip) + 4, _lib.stream_ptr()), "adam_step")
 
 
 # ------------------------------------------------------------------------------------------------ global gradient norm and clipping

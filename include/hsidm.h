@@ -486,9 +486,12 @@ int hsidm_gather_pack(const float* src, const int32_t* idx, int64_t n, void* out
 int hsidm_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
                     int step, float grad_scale, const float* coef_dev, void* stream);
 /* hsidm_adam_step with the gradient further scaled by *clip_dev (hsidm_grad_norm's out2 + 1): clipping without a pass over the
- * gradients of its own.  clip_dev NULL: hsidm_adam_step. */
+ * gradients of its own.  clip_dev NULL: hsidm_adam_step.  Both take 1 - beta of the fp32 betas they are given (1.3e-5 off at 0.999):
+ * hsidm_adam_step_f64 takes the rates in 64 bits, as torch.optim.Adam does, and is otherwise the same. */
 int hsidm_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
                             int step, float grad_scale, const float* coef_dev, const float* clip_dev, void* stream);
+int hsidm_adam_step_f64(float* p, const float* g, float* m, float* v, int64_t n, double lr, double beta1, double beta2, double eps,
+                        int step, float grad_scale, const float* coef_dev, const float* clip_dev, void* stream);
 
 /* ---- global gradient norm and clipping (torch.nn.utils.clip_grad_norm_'s definition, 2-norm) -------------------------------
  * host_items (HOST memory, read before the call returns): n_items tensors of n elements each, dense, at their element's natural
