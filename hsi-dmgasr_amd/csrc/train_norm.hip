@@ -695,11 +695,14 @@ extern "C" int hsidm_adam_step_f64(float* p, const float* g, float* m, float* v,
     if (!p || !g || !m || !v || n <= 0 || (step <= 0 && !coef_dev)) return HSIDM_E_BADARG;
     const int st = step > 0 ? step : 1;
     const double bc1 = 1.0 - pow(beta1, st), bc2 = 1.0 - pow(beta2, st);
-    const int64_t blocks = ((n >> 2) + 255) / 256;
-    if (blocks > 0x7fffffff) return HSIDM_E_UNSUPPORTED;
-    hipLaunchKernelGGL(clip_dev ? &adam_kernel<true> : &adam_kernel<false>, dim3((unsigned)(blocks > 0 ? blocks : 1)), dim3(256), 0, (hipStream_t)stream, p, g, m, v, n,
-                       (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)(lr / bc1), (float)(1.0 / sqrt(bc2)), (float)eps,
-                       grad_scale, coef_dev, clip_dev);
+    // (a launch has at most 2^32 threads: beyond 2^32 parameters - 16 GB of each buffer - one launch per 2^32 of them)
+    constexpr int64_t kPiece = (int64_t)1 << 32;
+    for (int64_t at = 0; at < n; at += kPiece) {
+        const int64_t here = n - at < kPiece ? n - at : kPiece, blocks = ((here >> 2) + 255) / 256;
+        hipLaunchKernelGGL(clip_dev ? &adam_kernel<true> : &adam_kernel<false>, dim3((unsigned)(blocks > 0 ? blocks : 1)), dim3(256), 0, (hipStream_t)stream, p + at, g + at,
+                           m + at, v + at, here, (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)(lr / bc1),
+                           (float)(1.0 / sqrt(bc2)), (float)eps, grad_scale, coef_dev, clip_dev);
+    }
     return (int)hipGetLastError();
 }
 

@@ -58,3 +58,19 @@ def test_steps_with_the_shipped_betas_against_torch(dev):
     s = opt.state[ref]
     # 20 steps of at most eight roundings each, on sums of positive terms
     assert bool(((v.double() - s["exp_avg_sq"]).abs() <= 160 * 2.0 ** -24 * s["exp_avg_sq"]).all())
+
+
+@GPU
+@pytest.mark.parametrize("clipped", [False, True], ids=["plain", "clipped"])
+def test_more_than_32_bits_of_parameters(dev, clipped):
+    """2^32 + 7 parameters: every one is stepped once, at the launch's first and last elements and around 2^32."""
+    from hsi_dmgasr_amd import train_ops as T
+    n = 2 ** 32 + 7
+    p, m, v = (torch.zeros(n, device=dev) for _ in range(3))
+    g = torch.ones(n, device=dev)
+    clip = torch.tensor([1.0, 0.5], device=dev) if clipped else None
+    T.adam_step(p, g, m, v, 0.25, 0.5, 0.75, 1e-30, 1, clip=clip)     # m and v hold (1 - beta) g^k, exactly; the increment is lr
+    x = 0.5 if clipped else 1.0
+    for t, want in ((m, 0.5 * x), (v, 0.25 * x * x)):
+        assert float(t[0]) == want and float(t[-1]) == want and torch.equal(t[-1:].expand(n), t)
+    assert float(p[0]) == -0.25 and torch.equal(p[:1].expand(n), p)
