@@ -617,7 +617,7 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void a
 // ---- launches: one translation unit per element type (attn_packed_<type>.hip) ---------------------------------------------------
 // kind: which kernel; waves: 2 or 4 per workgroup (a tile is 32 rows per wave)
 enum { ATTN_FWD = 0, ATTN_BWD = 1 };
-struct AttnBwdPair { AttnBwdArgs kv, q; int kv_tiles, q_tiles; };
+struct AttnBwdPair { AttnBwdArgs kv, q; };
 template <typename T> int attn_launch(int kind, const void* args, int waves, int ntiles, hipStream_t s);
 extern template int attn_launch<bf16>(int, const void*, int, int, hipStream_t);
 extern template int attn_launch<f16>(int, const void*, int, int, hipStream_t);

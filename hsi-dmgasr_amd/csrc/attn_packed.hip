@@ -183,7 +183,6 @@ static int check_attn(const hsidm_attn_desc* d, int& es) {
     if (!(d->scale > 0.f) || !(d->scale < 1e30f)) return HSIDM_E_BADARG;
     if (!rows_ok(d->q, d->q_ts, d->q_hs, es) || !rows_ok(d->k, d->k_ts, d->k_hs, es) || !rows_ok(d->v, d->v_ts, d->v_hs, es)) return HSIDM_E_BADARG;
     if (!d->qtiles64 || !d->qtiles128 || !d->ktiles64 || !d->ktiles128 || d->n64 <= 0 || d->n128 <= 0 || d->longest <= 0 || !(d->pairs > 0)) return HSIDM_E_BADARG;
-    if ((int64_t)d->n64 * d->Hq > 0x7fffffff) return HSIDM_E_UNSUPPORTED;
     return 0;
 }
 static AttnTensor tensor(const void* p, int64_t ts, int64_t hs, int es) { return {(const char*)p, ts * es, hs * es}; }
@@ -295,7 +294,7 @@ extern "C" int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* 
     else if (d->prec == HSIDM_F16) launch_delta<f16>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
     else launch_delta<float>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
     const bool tall = p.kv.waves == 4;
-    AttnBwdPair pair = {a, a, p.kv.ntiles, p.q.ntiles};
+    AttnBwdPair pair = {a, a};
     pair.kv.splits = p.kv.splits; pair.kv.part = (float*)(ws + p.part_kv);
     pair.kv.tiles = (const AttnTile*)(tall ? d->ktiles128 : d->ktiles64);
     pair.q.splits = p.q.splits; pair.q.part = (float*)(ws + p.part_q);
