@@ -263,7 +263,8 @@ class SelfAttention(_HipModule):
         if self.qk_norm_rope:
             dim = in_channel // n_head
             if dim % 16 or dim > 256:
-                raise ValueError("hsidm: qk_norm_rope needs heads of a multiple of 16 channels up to 256, got %d" % dim)
+                raise ValueError("hsidm: qk_norm_rope needs heads of a multiple of 16 channels up to 256, got %d (n_head = %d over %d channels; in a "
+                                 "UNet: attn_n_head)" % (dim, n_head, in_channel))
             self.q_norm, self.k_norm = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.ones(dim))
         self.norm = nn.GroupNorm(norm_groups, in_channel)
         self.qkv = nn.Conv2d(in_channel, in_channel * 3, 1, bias=False)
@@ -328,12 +329,13 @@ class SelfAttention(_HipModule):
 
 
 class ResnetBlocWithAttn(_HipModule):
-    def __init__(self, dim, dim_out, *, noise_level_emb_dim=None, norm_groups=32, dropout=0, with_attn=False, qk_norm_rope=False):
+    def __init__(self, dim, dim_out, *, noise_level_emb_dim=None, norm_groups=32, dropout=0, with_attn=False, qk_norm_rope=False,
+                 n_head=1):
         super().__init__()
         self.with_attn = with_attn
         self.res_block = ResnetBlock(dim, dim_out, noise_level_emb_dim, norm_groups=norm_groups, dropout=dropout)
         if with_attn:
-            self.attn = SelfAttention(dim_out, norm_groups=norm_groups, qk_norm_rope=qk_norm_rope)
+            self.attn = SelfAttention(dim_out, n_head, norm_groups=norm_groups, qk_norm_rope=qk_norm_rope)
 
     def _run(self, x0, x1, film, precision):
         x = self.res_block._run(x0, x1, film, precision)
@@ -349,8 +351,13 @@ class ResnetBlocWithAttn(_HipModule):
 
 
 class UNet(_HipModule):
+    """Reference unet.py:169-259.  attn_n_head, attn_qk_norm_rope (not arguments of the reference's UNet, which builds one head and no
+    positions): handed to every SelfAttention.  Heads of more than 256 channels - the shipped network's layers have 512 - take neither the
+    norm and rotation nor maps of more than 1024 tokens: attn_n_head=2 does."""
+
     def __init__(self, in_channel=6, out_channel=3, inner_channel=32, norm_groups=32, channel_mults=(1, 2, 4, 8, 8),
-                 attn_res=(8), res_blocks=3, dropout=0, with_noise_level_emb=True, image_size=128, precision=None, attn_qk_norm_rope=False):
+                 attn_res=(8), res_blocks=3, dropout=0, with_noise_level_emb=True, image_size=128, precision=None, attn_qk_norm_rope=False,
+                 attn_n_head=1):
         super().__init__()
         if not with_noise_level_emb:
             # the reference cannot build this variant either: its ResnetBlock constructs nn.Linear(None, dim_out)
@@ -371,7 +378,7 @@ class UNet(_HipModule):
 
         def unit(cin, cout, attn):
             return ResnetBlocWithAttn(cin, cout, noise_level_emb_dim=emb, norm_groups=norm_groups, dropout=dropout,
-                                      with_attn=attn, qk_norm_rope=attn_qk_norm_rope)
+                                      with_attn=attn, qk_norm_rope=attn_qk_norm_rope, n_head=attn_n_head)
 
         # encoder: stem conv, then per level `res_blocks` units (+ a stride-2 conv between levels)
         width = inner_channel

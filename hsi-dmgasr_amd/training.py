@@ -43,13 +43,14 @@ class Trainer:
         if not isinstance(net, UNet):
             raise TypeError("hsidm: Trainer needs a GaussianDiffusion over hsi_dmgasr_amd's UNet")
         self.gd, self.net = gd, net
-        # what the hand-written backward pass covers is what the reference's UNet builds (unet.py:152,206: one attention head,
-        # additive FiLM); the two constructor variants its classes also accept have forward kernels only
+        # what the hand-written backward pass covers: what the reference's UNet builds (unet.py:152,206: one attention head, additive
+        # FiLM), and any number of heads where a layer always runs on the packed attention kernels; FeatureWiseAffine's other form and
+        # several heads on the one-head kernels' side have forward kernels only
         for u in net._res_units():
             if u.res_block.noise_func.use_affine_level:
                 raise NotImplementedError("hsidm: the training step has no adjoint for FeatureWiseAffine(use_affine_level=True)")
-            if u.with_attn and u.attn.n_head != 1:
-                raise NotImplementedError("hsidm: the training step has no adjoint for SelfAttention(n_head=%d); n_head must be 1"
+            if u.with_attn and u.attn.n_head != 1 and not u.attn.qk_norm_rope:
+                raise NotImplementedError("hsidm: the training step has no adjoint for SelfAttention(n_head=%d); n_head must be 1 without qk_norm_rope"
                                           % u.attn.n_head)
         self.precision = resolve_precision(precision if precision is not None else net.precision)
         if self.precision not in ("bf16", "fp32"):
