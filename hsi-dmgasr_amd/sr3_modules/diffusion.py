@@ -24,7 +24,7 @@ from torch import nn
 
 from .. import ops
 from ..precision import internal_names, resolve_precision, step_precision
-from .unet import UNet
+from .unet import UNet, holding
 
 
 def make_beta_schedule(schedule, n_timestep, linear_start=1e-4, linear_end=2e-2, cosine_s=8e-3):
@@ -64,6 +64,7 @@ class _GraphSlot:
         self.key, self.weights = key, weights
         self.x = self.cond = self.t_ptr = self.stored = self.zbuf = self.snap = None
         self.graphs, self.eager_done, self.pool = {}, set(), None
+        self.plans = {}            # (unet.holding)
         self.busy = True
 
 
@@ -157,9 +158,9 @@ class ReverseRun:
                 self.cond.copy_(cond)
         if slot is not None:
             slot.x, slot.cond, slot.t_ptr, slot.stored, slot.zbuf, slot.snap = self.x, self.cond, self.t_ptr, self.stored, self.zbuf, self.snap
-            self.graphs, self._eager_done = slot.graphs, slot.eager_done
+            self.graphs, self._eager_done, self._plans = slot.graphs, slot.eager_done, slot.plans
         else:
-            self.graphs, self._eager_done = {}, set()
+            self.graphs, self._eager_done, self._plans = {}, set(), {}
         self._pool = None if slot is None else slot.pool   # one private memory pool for every captured graph of this run (replays are serial)
         self.steps_done = 0
 
@@ -177,7 +178,7 @@ class ReverseRun:
 
     def _enqueue(self, precision=None):
         gd = self.gd
-        with internal_names():              # (the step's kernel set may be one of the policy's dithered sets: an internal name)
+        with internal_names(), holding(self._plans):      # (the step's kernel set may be one of the policy's dithered sets: an internal name)
             eps = gd._denoise(self.cond, self.x, self.t_ptr, self.modes[-1] if precision is None else precision)
         if self.zbuf is not None:
             self.zbuf.normal_()

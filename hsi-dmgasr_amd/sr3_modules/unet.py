@@ -14,6 +14,11 @@ for naming / loading / initialisation; the arithmetic runs in libhsidm.so on NHW
 
 There is no eager fallback: inputs must be ROCm tensors and the library must be built.
 """
+import collections
+import contextlib
+import threading
+import weakref
+
 import torch
 from torch import nn
 
@@ -247,12 +252,42 @@ class ResnetBlock(_HipModule):
         return ops.to_nchw(self._run(ops.to_nhwc(x, p), None, film, p), p)
 
 
+class MapPlan:
+    """What the packed attention of a batch of maps goes by, unpacked as (sequences, positions, axes): one sequence per image; (row, column) of
+    every token and their RotaryAxes with qk_norm_rope, else None."""
+
+    def __init__(self, sequences, positions, axes):
+        self._parts = (sequences, positions, axes)
+
+    def __iter__(self):
+        return iter(self._parts)
+
+    def __getitem__(self, i):
+        return self._parts[i]
+
+
+_held = threading.local()
+
+
+@contextlib.contextmanager
+def holding(plans):
+    """Keeps the MapPlans that are used inside in `plans` (a dict): a captured step addresses their tables, and whoever owns its graph
+    owns them with it."""
+    outer, _held.plans = getattr(_held, "plans", None), plans
+    try:
+        yield plans
+    finally:
+        _held.plans = outer
+
+
 class SelfAttention(_HipModule):
     """Reference unet.py:114-143.  Maps of more than 1024 tokens - the reference's own einsum has no limit - run on the packed attention
     kernels (ops.attention_packed), which store nothing of size tokens^2; heads up to 256 channels there.
 
     qk_norm_rope (not in the reference; default off): queries and keys of every head pass an RMS norm (weights q_norm, k_norm) and are
     rotated by their pixel's row and column, half of the pairs each (ops.qk_norm_rope) - the only position information in the layer."""
+
+    MAPS_KEPT = 16                 # map shapes whose plans a layer keeps on its own account (about nine bytes a token each)
 
     def __init__(self, in_channel, n_head=1, norm_groups=32, *, qk_norm_rope=False):
         super().__init__()
@@ -270,20 +305,29 @@ class SelfAttention(_HipModule):
         self.qkv = nn.Conv2d(in_channel, in_channel * 3, 1, bias=False)
         self.out = nn.Conv2d(in_channel, in_channel, 1)
         self._cache = _PackCache()
-        self._maps = {}
+        self._no_plans()
+
+    def _no_plans(self):
+        # every plan that is alive; the latest shapes' ones; those of captures that nobody holds() for
+        self._maps, self._recent, self._pinned = weakref.WeakValueDictionary(), collections.OrderedDict(), {}
 
     def __getstate__(self):                            # (copies and checkpoints make their own plans, where they are)
-        return {**self.__dict__, "_maps": {}}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_maps", "_recent", "_pinned")}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._no_plans()
 
     def packed(self, tokens):
         """Does a map of that many tokens run on the packed attention kernels?"""
         return self.qk_norm_rope or tokens > 1024
 
     def map_plan(self, B, H, W, device):
-        """(sequences, positions, axes) of a batch of maps, kept per shape for good (captured steps hold their addresses; about nine bytes
-        a token): one sequence per image; (row, column) of every token."""
+        """The MapPlan of a batch of maps.  The plans of the last MAPS_KEPT shapes are kept; one that a captured step goes by for as long as
+        the step (see holding), or for good where the capture is a caller's own."""
         key = (B, H, W, device)
         plan = self._maps.get(key)
+        capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
         if plan is None:
             seqs, pos, axes = ops.PackedSequences([H * W] * B, device=device), None, None
             if self.qk_norm_rope:
@@ -291,7 +335,19 @@ class SelfAttention(_HipModule):
                 pos = grid.reshape(1, H * W, 2).expand(B, -1, -1).reshape(-1, 2).contiguous().to(device)
                 dim = self.q_norm.shape[0]
                 axes = ops.RotaryAxes((dim // 4, dim // 4), dim, device=device)
-            plan = self._maps[key] = (seqs, pos, axes)
+            plan = self._maps[key] = MapPlan(seqs, pos, axes)
+        self._recent[key] = plan
+        self._recent.move_to_end(key)
+        if len(self._recent) > self.MAPS_KEPT and not capturing:
+            if device.type == "cuda":
+                torch.cuda.synchronize(device)         # (another stream's launches may still read the tables; building new ones waits as well)
+            while len(self._recent) > self.MAPS_KEPT:
+                self._recent.popitem(last=False)
+        plans = getattr(_held, "plans", None)
+        if plans is not None:
+            plans[id(plan)] = plan
+        elif capturing:
+            self._pinned[key] = plan
         return plan
 
     def heads(self, qkv):

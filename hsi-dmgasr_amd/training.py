@@ -29,7 +29,7 @@ from torch import nn
 from . import ops
 from . import train_ops as T
 from .precision import resolve_precision
-from .sr3_modules.unet import Block, Downsample, ResnetBlocWithAttn, UNet, Upsample
+from .sr3_modules.unet import Block, Downsample, ResnetBlocWithAttn, UNet, Upsample, holding
 
 
 _NOTICE_DONE = False
@@ -79,6 +79,7 @@ class Trainer:
         self._defer_obj, self._defer = None, None
         self._g, self._g_active = None, False          # captured step (optimize_parameters): state, capturing / replaying
         self._eager_shape = None                       # batch shape of the LAST eager step (what every workspace is sized for)
+        self._plans = {}                               # the attention plans of that step (unet.holding): the captured step goes by them too
         self.dev = next(net.parameters()).device
         self._check_device()
         self._flatten()
@@ -737,7 +738,9 @@ class Trainer:
             # take pointers to (split-K and deferred-reduction workspaces, FiLM buffers, offset tables, LDS caps) and prunes the
             # packed layouts for this shape.  The reference's DataLoader has no drop_last: a partial last batch drops the graph,
             # runs eagerly, and the next full batch runs eagerly once more before it is captured again.
-            loss = self.loss_and_grads(data)
+            self._plans = {}
+            with holding(self._plans):
+                loss = self.loss_and_grads(data)
             self.optimizer_step()
             self._eager_shape = shape_key
             return loss
@@ -746,7 +749,7 @@ class Trainer:
                      gamma=torch.zeros(b, dtype=torch.float32, device=self.dev), key=torch.zeros(1, dtype=torch.int64, device=self.dev),
                      coef=torch.zeros(2, dtype=torch.float32, device=self.dev),
                      h_gamma=torch.zeros(b, dtype=torch.float32).pin_memory(), h_key=torch.zeros(1, dtype=torch.int64).pin_memory(),
-                     h_coef=torch.zeros(2, dtype=torch.float32).pin_memory(), graph=None, loss=None)
+                     h_coef=torch.zeros(2, dtype=torch.float32).pin_memory(), graph=None, loss=None, plans=self._plans)
             self._g = g
         g = self._g
         # ---- host side of the iteration: draws, counters, staging copies (stream-ordered ahead of the replay)
@@ -775,7 +778,7 @@ class Trainer:
             graph = torch.cuda.CUDAGraph()
             self._g_active = True
             try:
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph), holding(g["plans"]):
                     g["loss"] = self._captured_body(g)
             finally:
                 self._g_active = False
