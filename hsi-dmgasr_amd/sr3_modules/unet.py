@@ -315,7 +315,7 @@ class SelfAttention(_HipModule):
         return {k: v for k, v in self.__dict__.items() if k not in ("_maps", "_recent", "_pinned")}
 
     def __setstate__(self, state):
-        super().__setstate__(state)
+        super().__setstate__({"qk_norm_rope": False, **state})      # (a module pickled before the option)
         self._no_plans()
 
     def packed(self, tokens):

@@ -121,3 +121,17 @@ def test_a_callers_own_capture(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+
+
+def test_a_layer_pickled_before_it_had_plans():
+    """A whole-module checkpoint of an earlier build: no plans, no option."""
+    from hsi_dmgasr_amd.sr3_modules import unet
+    a = unet.SelfAttention(64)
+    old = {k: v for k, v in a.__dict__.items() if k not in ("_maps", "_recent", "_pinned", "qk_norm_rope")}
+    b = unet.SelfAttention.__new__(unet.SelfAttention)
+    b.__setstate__(old)
+    assert not b.packed(1024) and b.packed(1025) and b.map_plan(1, 33, 32, torch.device("cpu"))[0].lengths == (1056,)
+    # the build before this one kept a dict of tuples there
+    c = unet.SelfAttention.__new__(unet.SelfAttention)
+    c.__setstate__({**old, "qk_norm_rope": False, "_maps": {}})
+    assert c.map_plan(1, 33, 32, torch.device("cpu")) is c.map_plan(1, 33, 32, torch.device("cpu"))
