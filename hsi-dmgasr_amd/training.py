@@ -38,7 +38,7 @@ _NOTICE_DONE = False
 class Trainer:
     def __init__(self, gd, lr=1e-5, betas=(0.9, 0.999), eps=1e-8, precision=None, dropout_seed=0, bucket_bytes=64 << 20, max_grad_norm=None):
         """max_grad_norm: clip the gradient's global 2-norm to this before Adam (None, as the reference: no clipping); the norm of the
-        last step is left in ``last_grad_norm``."""
+        last step is left in ``last_grad_norm`` (None while nothing is clipped)."""
         net = gd.denoise_fn
         if not isinstance(net, UNet):
             raise TypeError("hsidm: Trainer needs a GaussianDiffusion over hsi_dmgasr_amd's UNet")
@@ -95,6 +95,8 @@ class Trainer:
         if value is not None and not float(value) > 0:
             raise ValueError("hsidm: max_grad_norm must be positive or None, got %r" % (value,))
         self._max_grad_norm = None if value is None else float(value)
+        if value is None:
+            self.last_grad_norm = None                 # (no step from here on has one)
         self._g = None                                 # a captured step has the bound baked in: the next call captures again
 
     def _check_device(self):
