@@ -136,8 +136,11 @@ static int tile_rows(int D, int es) { return row_bytes(D, es) <= 256 ? 64 : 32; 
 //   tiles of equal work: rounds of resident workgroups times a share's steps;
 //   unequal ones (causal, ragged; heaviest first): all work at the full rate, and 0.45 of the longest share at the end, alone;
 //   plus the shares' partial sums, written in fp32 and read again.
-// The rates are what the kernels reach (a step of the measured cases comes out within 15 %); shares stay at four steps or more.
-struct Walk { int resident, products; bool kv; };            // workgroups of four waves per CU (by registers), matrix products per tile pair
+// The rates and `resident` are constants of the estimate, fitted to the shares that measured best on a handful of cases when the forward
+// kernel took 165 registers at D = 64; they decide the number of shares and nothing else.  They are not what the kernels have today: registers
+// allow four forward workgroups of four waves at rows of 128 bytes (three are counted) and three at 256 in the 16-bit types (two), and the
+// query-gradient walk runs beside the key walk, two at most (three are counted at 128 bytes).  Shares stay at four steps or more.
+struct Walk { int resident, products; bool kv; };            // workgroups of four waves per CU, matrix products per tile pair
 // waves: 0 to choose, 2 or 4 to go with another kernel's tiles
 static Cut cut_work(const hsidm_attn_desc* d, int es, const Walk& k, int waves) {
     const int heads = k.kv ? d->Hk : d->Hq, walks = k.kv ? d->Hq / d->Hk : 1, rows = tile_rows(d->D, es), width = row_bytes(d->D, es) / es;

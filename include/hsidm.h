@@ -231,7 +231,8 @@ int hsidm_attention(int prec, const void* qkv, void* out, int B, int N, int C, v
  * or more tokens - {first token of the sequence, its length, first row of the tile within it, 0} - n64 / n128 of them; qtiles: in the
  * order query tiles should start (most work first), ktiles: key tiles.  longest: the longest sequence.  The
  * tiles together cover every one of the T tokens (what a split leaves in a row that none covers is undefined).
- * Values of k and v must be finite where a LATER token of the same 128-row tile is masked out for an earlier one (0 * inf is NaN).
+ * Values of k and v must be finite where a LATER token of the same 128-row tile is masked out for an earlier one (0 * inf is NaN); in the
+ * backward pass so must q and dout of an EARLIER token of the tile, for the dk and dv of a later one.
  * out_lo (16-bit types; may be NULL): what rounding out to the type left behind, for the backward pass: rowsum(dout o out) from both is
  *   exact to fp32, and dq / dk are then as exact as rounding dS allows.
  * Backward: from out (+ out_lo), lse and dout, recomputing the scores: dq, dk, dv (strided like their tensors, apart from all that is read), dk / dv summed over the heads that
