@@ -361,16 +361,19 @@ __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 512 ? 2 : 1)) void a
 // Two kinds of workgroups recompute S and dP: one owns key tiles and walks the queries of every head that shares them (dK, dV: the sum over a group's
 // heads stays in registers), one owns query tiles and walks the keys (dQ).  Nothing is added atomically: results do not depend on order.
 // fp16: P and dS are stored to 11 bits with exponents down to 2^-14 only, and both shrink with the number of keys and the gradient's
-// size.  P is kept times 2^10 and dS times a power of two chosen from max |dO| and max |V| (|dP - delta| <= 2 |dO| |V|): neither
-// overflows, and underflow starts 2^10 and more lower.  bf16 has fp32's exponents and needs none of it.
+// size.  P is kept times 2^10 and dS times a power of two chosen from |dO| and |V| (|dP - delta| <= 2 |dO| |V|): neither overflows, and
+// underflow starts 2^10 and more lower.  dQ takes the power from its row's own |dO|; dK, a sum over rows, from the largest of the rows that see
+// the tile's keys; |V| is the sequence's largest.  (One power for a whole call lost a long sequence beside a short one whose gradients are 2^18
+// times as large.)  Only finite rows count: one with an infinity or a NaN has no finite gradient to scale.  bf16 has fp32's exponents and needs
+// none of it.
 struct AttnBwdArgs {
     AttnTensor q, k, v, dout, dq, dk, dv;
     const float *lse, *delta;        // [Hq][T]
-    const float* maxima;             // [nmax][2]: partial maxima of |dO|^2 and |V|^2 (fp16)
+    const float *top_do, *top_v;     // fp16, [Hk][T]: at a 64-row tile's first token, the largest |dO|^2 (over the group's heads) and |V|^2 of its rows
     float* part;                     // partial sums of split work: dQ [splits][T][Hq][D], or (dK | dV) [splits][2][T][Hk][D]
     const AttnTile* tiles;
     int64_t T;
-    int Hq, Hk, D, causal, splits, nmax;
+    int Hq, Hk, D, causal, splits;
     float scale;
 };
 
@@ -382,13 +385,18 @@ template <> struct GradScale<f16> {
     static constexpr bool on = true;
     static constexpr float p_shift = 10.f, p_back = 1.f / 1024.f;
 };
-// The power of two that dS = P' (dP - delta), P' = 2^10 P, is multiplied by.  The maxima are those of finite fp16 rows: at most 256 * 65504^2,
-// so that `top` is finite; it is zero only where every finite row of dO or of V is zero, and dS then is too.
-__device__ __forceinline__ float grad_factor(const float* maxima, int n, int lane) {
-    float a = 0.f, b = 0.f;
-    for (int i = lane; i < n; i += 64) { a = fmaxf(a, maxima[2 * i]); b = fmaxf(b, maxima[2 * i + 1]); }
-    a = wave_max(a); b = wave_max(b);
-    const float top = 2048.f * sqrtf(a) * sqrtf(b);              // |P' (dP - delta)|
+__device__ __forceinline__ float finite_or_zero(float x) { return x < INFINITY ? x : 0.f; }      // (of a sum of squares: NaN compares false)
+
+// the largest of a sequence's 64-row tiles from row `from` (a tile's first) on; the same in every lane
+__device__ __forceinline__ float top_of_tiles(const float* top, int from, int len, int lane) {
+    float m = 0.f;
+    for (int64_t r = from + 64 * lane; r < len; r += 64 * 64) m = fmaxf(m, top[r]);
+    return wave_max(m);
+}
+// The power of two that dS = P' (dP - delta), P' = 2^10 P, is multiplied by, from |dO|^2 and |V|^2.  Those are of finite fp16 rows, at most
+// 256 * 65504^2 each, so that `top` is finite; it is zero only where dO or V is, and dS then is too.
+__device__ __forceinline__ float grad_factor(float do2, float v2) {
+    const float top = 2048.f * sqrtf(do2) * sqrtf(v2);           // |P' (dP - delta)|
     if (!(top > 0.f)) return 1.f;
     int e;
     frexpf(32768.f / top, &e);
@@ -428,7 +436,10 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnBwdArgs& a, char* lds, int
     for (int d = 0; d < ND; ++d) { zero16(dk[d]); zero16(dv[d]); }
     const float c = a.scale * kLog2e;
     float f = 1.f;
-    if constexpr (GradScale<T>::on) f = grad_factor(a.maxima, a.nmax, lane);
+    if constexpr (GradScale<T>::on) {
+        const int64_t first = kvh * a.T + tile.start;
+        f = grad_factor(top_of_tiles(a.top_do + first, a.causal ? tile.row0 : 0, len, lane), top_of_tiles(a.top_v + first, 0, len, lane));
+    }
     const Stage<T, DP, BQ, NW> qst(a.q.ts, pieces, wave, lane), gst(a.dout.ts, pieces, wave, lane);
     auto stage = [&](int w, int buf) __attribute__((always_inline)) {
         const int g = w / ntq, t = tq0 + w - g * ntq, head = kvh * group + g;
@@ -543,7 +554,16 @@ __device__ __forceinline__ void attn_bwd_q(const AttnBwdArgs& a, char* lds, int 
     for (int d = 0; d < ND; ++d) zero16(dq[d]);
     const float c = a.scale * kLog2e;
     float f = 1.f;
-    if constexpr (GradScale<T>::on) f = grad_factor(a.maxima, a.nmax, lane);
+    if constexpr (GradScale<T>::on) {                                // (this lane's row)
+        float sq = 0.f;
+#pragma unroll
+        for (int t = 0; t < R::STEPS; ++t) {
+            const auto x = __builtin_bit_cast(typename Elem<T>::x8, gf[t]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sq += (float)x[i] * (float)x[i];
+        }
+        f = grad_factor(finite_or_zero(both_halves_sum(sq)), top_of_tiles(a.top_v + kvh * a.T + tile.start, 0, len, lane));
+    }
     const Stage<T, DP, BN, NW> kst(a.k.ts, pieces, wave, lane), vst(a.v.ts, pieces, wave, lane);
     auto stage = [&](int t, int buf) __attribute__((always_inline)) {
         kst(kb, t * BN, len, lds + buf * 2 * TILE, wave);

@@ -66,63 +66,88 @@ __global__ __launch_bounds__(256) void attn_add_kernel(AttnSums sums, int64_t T_
 }
 
 // delta[h][t] = sum_d dO O per row, O with its rounding residual where the forward pass kept it (without it, delta's error is as large as
-// that of rounding dS and adds to it in dQ and dK: 1.55 ... 1.7 instead of 1.4 times the output's own rounding); fp16: also this workgroup's largest |dO|^2 and |V|^2 (GradScale) of
-// its finite rows - a row with an infinity or a NaN has no finite gradient to scale, and must not decide the scale of the others'.
-// `group` lanes, a power of two that covers a row's 16-byte pieces, share a row.
+// that of rounding dS and adds to it in dQ and dK: 1.55 ... 1.7 instead of 1.4 times the output's own rounding).  `group` lanes, a power of two
+// that covers a row's 16-byte pieces, share a row.
+struct DeltaRows {
+    AttnTensor dout, o;
+    const char* lo;
+    int pieces, group;
+};
+__device__ __forceinline__ float group_sum(float x, int group) {
+    for (int s = group >> 1; s > 0; s >>= 1) x += __shfl_xor(x, s, 64);
+    return x;
+}
+// one row's dO . O, and this lane's share of |dO|^2
+template <typename T>
+__device__ __forceinline__ float delta_row(const DeltaRows& a, int64_t token, int head, int sub, bool live, float& sq) {
+    constexpr int E = 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(E)));
+    float dot = 0.f;
+    sq = 0.f;
+    if (live && sub < a.pieces) {
+        const vec x = *reinterpret_cast<const vec*>(a.dout.p + token * a.dout.ts + head * a.dout.hs + sub * 16);
+        const vec y = *reinterpret_cast<const vec*>(a.o.p + token * a.o.ts + head * a.o.hs + sub * 16);
+#pragma unroll
+        for (int k = 0; k < E; ++k) { dot += (float)x[k] * (float)y[k]; sq += (float)x[k] * (float)x[k]; }
+        if (sizeof(T) == 2 && a.lo) {
+            const vec z = *reinterpret_cast<const vec*>(a.lo + token * a.o.ts + head * a.o.hs + sub * 16);
+#pragma unroll
+            for (int k = 0; k < E; ++k) dot += (float)x[k] * (float)z[k];
+        }
+    }
+    return group_sum(dot, a.group);
+}
+
 constexpr int kDeltaBlocks = 512;
 
-__device__ __forceinline__ float finite_or_zero(float x) { return x < INFINITY ? x : 0.f; }      // (of a sum of squares: NaN compares false)
-
 template <typename T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnTensor dout, AttnTensor o, const char* __restrict__ lo, AttnTensor v, int64_t T_, int Hq, int Hk, int pieces, int group,
-                                                         float* __restrict__ delta, float* __restrict__ maxima) {
+__global__ __launch_bounds__(256) void attn_delta_kernel(DeltaRows a, int64_t T_, int Hq, float* __restrict__ delta) {
+    const int sub = threadIdx.x & (a.group - 1), per = 256 / a.group;
+    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < T_ * Hq; r0 += (int64_t)gridDim.x * per) {
+        const int64_t r = r0 + threadIdx.x / a.group, token = r / Hq;
+        const int head = (int)(r - token * Hq);
+        float sq;
+        const float dot = delta_row<T>(a, token, head, sub, r < T_ * Hq, sq);
+        if (r < T_ * Hq && sub == 0) delta[head * T_ + token] = dot;
+    }
+}
+
+// fp16: a workgroup per (64-row tile, key head), which also leaves the largest |dO|^2 and |V|^2 of the tile's finite rows (GradScale) at the
+// tile's first token.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_delta_tiles_kernel(DeltaRows a, AttnTensor v, const AttnTile* __restrict__ tiles, int64_t T_, int g, float* __restrict__ delta,
+                                                               float* __restrict__ top_do, float* __restrict__ top_v) {
     constexpr int E = 16 / (int)sizeof(T);
     typedef T vec __attribute__((ext_vector_type(E)));
     __shared__ float red[2][4];
-    const int sub = threadIdx.x & (group - 1), per = 256 / group;
-    auto sum = [&](float x) __attribute__((always_inline)) {
-        for (int s = group >> 1; s > 0; s >>= 1) x += __shfl_xor(x, s, 64);
-        return x;
-    };
+    const AttnTile tile = tiles[blockIdx.x];
+    const int kvh = blockIdx.y, sub = threadIdx.x & (a.group - 1), per = 256 / a.group, rows = min(64, tile.len - tile.row0);
+    const int64_t first = (int64_t)tile.start + tile.row0;
     float ma = 0.f, mb = 0.f;
-    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < T_ * Hq; r0 += (int64_t)gridDim.x * per) {
-        const int64_t r = r0 + threadIdx.x / group, token = r / Hq;
-        const int head = (int)(r - token * Hq);
-        float dot = 0.f, sq = 0.f;
-        if (r < T_ * Hq && sub < pieces) {
-            const vec x = *reinterpret_cast<const vec*>(dout.p + token * dout.ts + head * dout.hs + sub * 16);
-            const vec y = *reinterpret_cast<const vec*>(o.p + token * o.ts + head * o.hs + sub * 16);
-#pragma unroll
-            for (int k = 0; k < E; ++k) { dot += (float)x[k] * (float)y[k]; sq += (float)x[k] * (float)x[k]; }
-            if (sizeof(T) == 2 && lo) {
-                const vec z = *reinterpret_cast<const vec*>(lo + token * o.ts + head * o.hs + sub * 16);
-#pragma unroll
-                for (int k = 0; k < E; ++k) dot += (float)x[k] * (float)z[k];
-            }
-        }
-        dot = sum(dot);
-        if (GradScale<T>::on) ma = fmaxf(ma, finite_or_zero(sum(sq)));
-        if (r < T_ * Hq && sub == 0) delta[head * T_ + token] = dot;
+    for (int r0 = 0; r0 < rows * g; r0 += per) {                     // (a token's heads one behind the other)
+        const int r = r0 + threadIdx.x / a.group, row = r / g, head = kvh * g + (r - row * g);
+        const bool live = row < rows;
+        float sq;
+        const float dot = delta_row<T>(a, first + row, head, sub, live, sq);
+        ma = fmaxf(ma, finite_or_zero(group_sum(sq, a.group)));
+        if (live && sub == 0) delta[head * T_ + first + row] = dot;
     }
-    if constexpr (GradScale<T>::on) {
-        for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < T_ * Hk; r0 += (int64_t)gridDim.x * per) {
-            const int64_t r = r0 + threadIdx.x / group, token = r / Hk;
-            const int head = (int)(r - token * Hk);
-            float sq = 0.f;
-            if (r < T_ * Hk && sub < pieces) {
-                const vec x = *reinterpret_cast<const vec*>(v.p + token * v.ts + head * v.hs + sub * 16);
+    for (int r0 = 0; r0 < rows; r0 += per) {
+        const int row = r0 + threadIdx.x / a.group;
+        float sq = 0.f;
+        if (row < rows && sub < a.pieces) {
+            const vec x = *reinterpret_cast<const vec*>(v.p + (first + row) * v.ts + kvh * v.hs + sub * 16);
 #pragma unroll
-                for (int k = 0; k < E; ++k) sq += (float)x[k] * (float)x[k];
-            }
-            mb = fmaxf(mb, finite_or_zero(sum(sq)));
+            for (int k = 0; k < E; ++k) sq += (float)x[k] * (float)x[k];
         }
-        ma = wave_max(ma); mb = wave_max(mb);
-        if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = ma; red[1][threadIdx.x >> 6] = mb; }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            maxima[2 * blockIdx.x] = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-            maxima[2 * blockIdx.x + 1] = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-        }
+        mb = fmaxf(mb, finite_or_zero(group_sum(sq, a.group)));
+    }
+    ma = wave_max(ma); mb = wave_max(mb);
+    if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = ma; red[1][threadIdx.x >> 6] = mb; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        top_do[kvh * T_ + first] = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+        top_v[kvh * T_ + first] = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
     }
 }
 
@@ -197,29 +222,32 @@ static int launch(int prec, int kind, const void* args, const Cut& c, hipStream_
 }
 static unsigned blocks_for(int64_t n) { const int64_t b = (n + 255) / 256; return (unsigned)(b < 65536 ? b : 65536); }
 
-struct BwdPlan { Cut q, kv; int64_t delta, maxima, part_kv, part_q, bytes; int nmax; };
+struct BwdPlan { Cut q, kv; int64_t delta, top_do, top_v, part_kv, part_q, bytes; };
 static BwdPlan bwd_plan(const hsidm_attn_desc* d, int es) {
     BwdPlan p;
     p.kv = cut_keys(d, es);
     p.q = cut_queries(d, es, 3, p.kv.waves);                          // (one launch: one tile height)
-    int group = 1;
-    while (group < d->D * es / 16) group *= 2;
-    const int64_t rows = d->T * d->Hq, blocks = (rows * group + 255) / 256;
-    p.nmax = (int)(blocks < kDeltaBlocks ? blocks : kDeltaBlocks);
+    const int64_t top = d->prec == HSIDM_F16 ? up16(d->T * d->Hk * 4) : 0;
     p.delta = 0;
-    p.maxima = up16(rows * 4);
-    p.part_kv = p.maxima + up16((int64_t)p.nmax * 8);
+    p.top_do = up16(d->T * d->Hq * 4);
+    p.top_v = p.top_do + top;
+    p.part_kv = p.top_v + top;
     p.part_q = p.part_kv + (p.kv.splits > 1 ? (int64_t)p.kv.splits * 2 * d->T * d->Hk * d->D * 4 : 0);
     p.bytes = p.part_q + (p.q.splits > 1 ? (int64_t)p.q.splits * d->T * d->Hq * d->D * 4 : 0);
     return p;
 }
 
 template <typename T>
-static void launch_delta(const AttnTensor& dout, const AttnTensor& o, const void* lo, const AttnTensor& v, const hsidm_attn_desc* d, int pieces, int nmax, float* delta,
-                         float* maxima, hipStream_t s) {
-    int group = 1;
-    while (group < pieces) group *= 2;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_delta_kernel<T>), dim3(nmax), dim3(256), 0, s, dout, o, (const char*)lo, v, d->T, d->Hq, d->Hk, pieces, group, delta, maxima);
+static void launch_delta(const DeltaRows& a, const hsidm_attn_desc* d, float* delta, hipStream_t s) {
+    const int64_t blocks = (d->T * d->Hq * a.group + 255) / 256;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_delta_kernel<T>), dim3((unsigned)(blocks < kDeltaBlocks ? blocks : kDeltaBlocks)), dim3(256), 0, s, a, d->T, d->Hq, delta);
+}
+// (at most 2^32 threads along an axis: more tiles go in several launches)
+static void launch_delta_f16(const DeltaRows& a, const AttnTensor& v, const hsidm_attn_desc* d, float* delta, float* top_do, float* top_v, hipStream_t s) {
+    const AttnTile* tiles = (const AttnTile*)d->qtiles64;
+    for (int64_t left = d->n64, most = 0xffffffffLL / 256; left > 0; left -= most, tiles += most)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attn_delta_tiles_kernel<f16>), dim3((unsigned)(left < most ? left : most), d->Hk), dim3(256), 0, s, a, v, tiles, d->T, d->Hq / d->Hk,
+                           delta, top_do, top_v);
 }
 template <typename T>
 static void launch_add(const AttnSums& sums, int n, int heads, int64_t T_, int D, hipStream_t s) {
@@ -283,19 +311,19 @@ extern "C" int hsidm_attention_packed_bwd(const hsidm_attn_desc* d, const void* 
     const BwdPlan p = bwd_plan(d, es);
     if (!rows_ok(workspace, 0, 0, 4) || workspace_bytes < p.bytes) return HSIDM_E_BADARG;
     char* ws = (char*)workspace;
-    float *delta = (float*)(ws + p.delta), *maxima = (float*)(ws + p.maxima);
+    float *delta = (float*)(ws + p.delta), *top_do = (float*)(ws + p.top_do), *top_v = (float*)(ws + p.top_v);
     hipStream_t s = (hipStream_t)stream;
     AttnBwdArgs a;
     a.q = tensor(d->q, d->q_ts, d->q_hs, es); a.k = tensor(d->k, d->k_ts, d->k_hs, es); a.v = tensor(d->v, d->v_ts, d->v_hs, es);
     a.dout = tensor(dout, do_ts, do_hs, es);
     a.dq = tensor(dq, dq_ts, dq_hs, es); a.dk = tensor(dk, dk_ts, dk_hs, es); a.dv = tensor(dv, dv_ts, dv_hs, es);
-    a.lse = lse; a.delta = delta; a.maxima = maxima;
-    a.T = d->T; a.Hq = d->Hq; a.Hk = d->Hk; a.D = d->D; a.causal = d->causal; a.nmax = p.nmax; a.scale = d->scale;
-    const AttnTensor o = tensor(out, (int64_t)d->Hq * d->D, d->D, es);
-    const int pieces = d->D * es / 16;
-    if (d->prec == HSIDM_BF16) launch_delta<bf16>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
-    else if (d->prec == HSIDM_F16) launch_delta<f16>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
-    else launch_delta<float>(a.dout, o, out_lo, a.v, d, pieces, p.nmax, delta, maxima, s);
+    a.lse = lse; a.delta = delta; a.top_do = top_do; a.top_v = top_v;
+    a.T = d->T; a.Hq = d->Hq; a.Hk = d->Hk; a.D = d->D; a.causal = d->causal; a.scale = d->scale;
+    DeltaRows rows = {a.dout, tensor(out, (int64_t)d->Hq * d->D, d->D, es), (const char*)out_lo, d->D * es / 16, 1};
+    while (rows.group < rows.pieces) rows.group *= 2;
+    if (d->prec == HSIDM_BF16) launch_delta<bf16>(rows, d, delta, s);
+    else if (d->prec == HSIDM_F16) launch_delta_f16(rows, a.v, d, delta, top_do, top_v, s);
+    else launch_delta<float>(rows, d, delta, s);
     const bool tall = p.kv.waves == 4;
     AttnBwdPair pair = {a, a};
     pair.kv.splits = p.kv.splits; pair.kv.part = (float*)(ws + p.part_kv);

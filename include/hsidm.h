@@ -236,7 +236,7 @@ int hsidm_attention(int prec, const void* qkv, void* out, int B, int N, int C, v
  * out_lo (16-bit types; may be NULL): what rounding out to the type left behind, for the backward pass: rowsum(dout o out) from both is
  *   exact to fp32, and dq / dk are then as exact as rounding dS allows.
  * Backward: from out (+ out_lo), lse and dout, recomputing the scores: dq, dk, dv (strided like their tensors, apart from all that is read), dk / dv summed over the heads that
- * share them; no atomics, fixed order (fp16: P and dS are scaled by one power of two per call, from the largest |dout|^2 |v|^2 among the finite rows).  Workspaces: the _workspace_bytes functions (forward: 0 unless the keys are split), 16-byte aligned. */
+ * share them; no atomics, fixed order (fp16: P and dS are scaled by powers of two from the largest |dout|^2 |v|^2 among a sequence's finite rows).  Workspaces: the _workspace_bytes functions (forward: 0 unless the keys are split), 16-byte aligned. */
 typedef struct hsidm_attn_tile { int32_t start, len, row0, reserved; } hsidm_attn_tile;
 typedef struct hsidm_attn_desc {
     const void *q, *k, *v;

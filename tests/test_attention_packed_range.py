@@ -66,3 +66,76 @@ def test_gradients_beside_a_sequence_with_infinities(dev, where, bad):
         assert bool(torch.isfinite(g[keep]).all()), name
         close(g[keep], want[name][keep], want["m" + name][keep], 4, name)
     close(o[keep], want["o"][keep], want["mo"][keep], 2, "out")
+
+
+@GPU
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("below", [0, 10, 14, 18])
+def test_gradients_far_smaller_than_another_sequences(dev, below, causal):
+    """fp16 gradients of a scaled loss: one short sequence at 8192, a long one 2^below times smaller (a mean over its own length, say) -
+    all of them normal numbers.  The scale that dS is held at is the sequence's own."""
+    from hsi_dmgasr_amd import ops
+    from hsi_dmgasr_amd import train_ops as Tr
+    lengths = [64, 2100, 33]
+    q, k, v, do = make(dev, lengths, 4, 2, 64, torch.float16, seed=2, gain=0.5)
+    do = do.float() * 8192.0
+    do[64:2164] *= 2.0 ** -below
+    do[2164:] *= 2.0 ** -below / 4
+    do = do.clamp(-6e4, 6e4).half()
+    seqs = ops.PackedSequences(lengths, device=dev)
+    o, saved = ops.attention_packed(q, k, v, seqs, causal=causal, want_lse=True)
+    got = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, causal=causal)
+    want, _ = plain64(q, k, v, lengths, causal, 0.125, do)
+    first = 0
+    for n in lengths:
+        to = slice(first, first + n)
+        first += n
+        for name, g in zip(("dq", "dk", "dv"), got):
+            # per sequence, as a whole: within 4 half-steps of the type (the bound of test_long_rows_and_gradient_sizes), and half a subnormal
+            # step a value for those that the type cannot hold as normal numbers
+            w = want[name][to]
+            floor = torch.finfo(torch.float16).smallest_normal * torch.finfo(torch.float16).eps * w.numel() ** 0.5
+            err = float((g[to].double() - w).norm())
+            assert err <= 4 * 2.0 ** -11 * float(w.norm()) + floor, (name, n, err / float(w.norm()) * 2 ** 11)
+
+
+@GPU
+def test_gradients_of_rows_far_smaller_than_others_of_their_sequence(dev):
+    """One sequence, causal: the first rows' gradients are 2^16 times the last ones'.  Each row's dQ is held at its own scale."""
+    from hsi_dmgasr_amd import ops
+    from hsi_dmgasr_amd import train_ops as Tr
+    n = 700
+    q, k, v, do = make(dev, [n], 2, 1, 64, torch.float16, seed=3, gain=0.5)
+    do = do.float() * 4096.0
+    do[300:] *= 2.0 ** -16
+    do = do.half()
+    seqs = ops.PackedSequences([n], device=dev)
+    o, saved = ops.attention_packed(q, k, v, seqs, causal=True, want_lse=True)
+    got = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, causal=True)
+    want, _ = plain64(q, k, v, [n], True, 0.125, do)
+    for name, g, to in (("dq", got[0], slice(300, n)), ("dq", got[0], slice(0, 300)), ("dk", got[1], slice(384, n)), ("dv", got[2], slice(300, n))):
+        w = want[name][to]               # (dk of keys behind row 384, a tile's edge: every query that sees them is a small one)
+        floor = torch.finfo(torch.float16).smallest_normal * torch.finfo(torch.float16).eps * w.numel() ** 0.5
+        err = float((g[to].double() - w).norm())
+        assert err <= 4 * 2.0 ** -11 * float(w.norm()) + floor, (name, to, err / float(w.norm()) * 2 ** 11)
+
+
+@GPU
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 3e4], ids=str)
+def test_other_sequences_gradients_never_matter(dev, bad):
+    """Whatever one sequence's tensors hold, the others' fp16 gradients are the same to the last bit."""
+    from hsi_dmgasr_amd import ops
+    from hsi_dmgasr_amd import train_ops as Tr
+    lengths = [50, 30, 70, 200]
+    q, k, v, do = make(dev, lengths, 4, 2, 64, torch.float16, seed=4)
+    seqs = ops.PackedSequences(lengths, device=dev)
+    for causal in (False, True):
+        o, saved = ops.attention_packed(q, k, v, seqs, causal=causal, want_lse=True)
+        want = Tr.attention_packed_bwd(do, q, k, v, o, saved, seqs, causal=causal)
+        qb, kb, vb, db = (x.clone() for x in (q, k, v, do))
+        for x in (qb, kb, vb, db):
+            x[60, :, 3] = bad
+        ob, sb = ops.attention_packed(qb, kb, vb, seqs, causal=causal, want_lse=True)
+        got = Tr.attention_packed_bwd(db, qb, kb, vb, ob, sb, seqs, causal=causal)
+        keep = torch.cat([torch.arange(50), torch.arange(80, 350)]).to(dev)
+        assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, want))
