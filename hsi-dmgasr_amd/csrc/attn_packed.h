@@ -249,8 +249,8 @@ template <> struct ProbScale<f16> { static constexpr float shift = 11.f, lazy = 
 // two hardly overlap, neither is full, and of the 182 us a pass takes, 127 would be those two in strict turn at 2.4 GHz (73 if they overlapped).
 // fp16, 2 x 16384 tokens, one head of 64: 187 us, 735 TFLOP/s; bf16 causal, 20115 tokens in six sequences, 16 / 4 heads of 128: 502 ... 530 us,
 // 880 ... 930 TFLOP/s of the pairs that count; fp32 (exact products, peak 157), 2 x 4096 tokens of 128: 154 us, 112 TFLOP/s.  D = 256, 8 x 2048
-// tokens, 8 heads: bf16 303 us, fp16 318 (907 and 864 TFLOP/s); fp32, 2 x 4096, one head: 313, 110.  Head sizes between the widths of 32, 64, 128 and 256 do
-// the products of the next one: 8 x 2048 tokens, 16 heads, bf16: D = 80 315 us, 96 324, 128 350.
+// tokens, 8 heads: bf16 297 us, fp16 311 (925 and 883 TFLOP/s); fp32, 2 x 4096, one head: 312, 110.  Head sizes between the widths of 32, 64, 128 and 256 do
+// the products of the next one: 8 x 2048 tokens, 16 heads, bf16: D = 80 313 us, 96 322, 128 334 ... 350.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 512 ? 2 : 1)) void attn_fwd_kernel(AttnFwdArgs a) {
     typedef Row<T, DP> R;
@@ -622,11 +622,11 @@ __device__ __forceinline__ void attn_bwd_q(const AttnBwdArgs& a, char* lds, int 
 // free - a launch of its own would begin when the last of them ends (fp16 4 x 256 tokens, 8 heads of 64: 13 us instead of 25; bf16 causal,
 // 10739 tokens in five sequences, 8 / 2 heads of 128: 304 us instead of 412).
 // Bound by the matrix pipe together with the vector work and the LDS reads between its instructions (four products per pair of tiles read
-// 32 KB a wave at D = 128, as long as they multiply).  8 x 2048 tokens, 16 heads, bf16: D = 128 1095 ... 1114 us, D = 64 529 ... 575 us - 870 and 870
+// 32 KB a wave at D = 128, as long as they multiply).  8 x 2048 tokens, 16 heads, bf16: D = 128 1086 ... 1114 us, D = 64 529 ... 575 us - 875 and 870
 // TFLOP/s of the seven products that run (two of them recompute S and dP); fp32, 2 x 4096 tokens of 128: 528 ... 540 us, 114 TFLOP/s.
-// Registers: D = 128 in the 16-bit types spills 10 ... 20 of them (28 ... 52 bytes of scratch a lane), fp32 D = 64 two or three, fp32 D = 256 65 ... 106 (184
-// ... 260 bytes); what that costs was not measured.  D = 256 recomputes the scores for either half of D and has one wave on a SIMD: 8 x 2048 tokens, 8
-// heads, bf16 1705 us, fp16 1809 (at D = 128 and 16 heads, as many products: 1114 and 1198); fp32, 2 x 4096, one head: 1348, 2.5 times D = 128.
+// Registers: D = 128 in the 16-bit types spills 10 ... 20 of them (28 ... 52 bytes of scratch a lane), fp32 D = 64 two or three, fp32 D = 256 65 ... 106 (168
+// ... 244 bytes); what that costs was not measured.  D = 256 recomputes the scores for either half of D and has one wave on a SIMD: 8 x 2048 tokens, 8
+// heads, bf16 1703 us, fp16 1763 (at D = 128 and 16 heads, as many products: 1086 and 1179); fp32, 2 x 4096, one head: 1347, 2.5 times D = 128.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (Row<T, DP>::BYTES <= 256 ? 2 : 1)) void attn_bwd_kernel(AttnBwdArgs kv, AttnBwdArgs q, int kv_blocks, int q_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
