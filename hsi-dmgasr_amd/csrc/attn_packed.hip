@@ -227,7 +227,7 @@ static BwdPlan bwd_plan(const hsidm_attn_desc* d, int es) {
     BwdPlan p;
     p.kv = cut_keys(d, es);
     p.q = cut_queries(d, es, 3, p.kv.waves);                          // (one launch: one tile height)
-    const int64_t top = d->prec == HSIDM_F16 ? up16(d->T * d->Hk * 4) : 0;
+    const int64_t top = es == 2 ? up16(d->T * d->Hk * 4) : 0;         // (one layout for the 16-bit types; fp16 uses it)
     p.delta = 0;
     p.top_do = up16(d->T * d->Hq * 4);
     p.top_v = p.top_do + top;
